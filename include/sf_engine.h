@@ -54,6 +54,9 @@ extern "C" {
 #define SF_ACT_NONE 0
 #define SF_ACT_SILU 1
 #define SF_ACT_GELU_TANH 2
+/* Gated SiLU, silu(v[n]) * v[N + n]: sf_gemm_grouped only (it reads 2 N
+ * weight rows for N outputs). */
+#define SF_ACT_SILU_GATE 3
 
 /* fp32 GEMM arithmetic.  ACCURATE (default) = 3xTF32 on tcgen05, the
  * replacement for non-TF32 cuBLAS SGEMM; FFMA = IEEE fp32 SIMT;
@@ -153,6 +156,84 @@ int32_t sf_linear_skinny_noalloc(int64_t M, int64_t N, int64_t K,
                                  const void* bias, int32_t bias_dtype,
                                  void* y, int64_t ldy, int32_t in_dtype, int32_t out_dtype,
                                  int32_t activation, void* stream);
+
+/* ───────────────────────── grouped products ───────────────────────── */
+
+/* One linear per group over rows grouped by expert:
+ *   C[i, :] = act(B[g] . A[r(i), :] + bias[g])
+ * for offsets[g] <= i < offsets[g + 1], with r(i) = rows[i], or i when rows
+ * is NULL.  offsets (device, [groups + 1], non-decreasing, in 0..M) and rows
+ * (device, [M], in 0..a_rows-1) are not read by the host: one launch whatever
+ * the group sizes are, empty groups included.  Row i of C that lies in no
+ * group is not written; an index outside 0..a_rows-1 reads a row of zeros;
+ * offsets outside 0..M are clamped.
+ *   B [groups][N][K] in the nn.Linear layout ([groups][2 N][K] for
+ *   SF_ACT_SILU_GATE: N gate rows, then N value rows), rows ldb apart and
+ *   groups b_stride apart; bias likewise, bias_stride apart, or NULL.
+ * 16-bit operands whose rows start on 16-byte boundaries run on the tensor
+ * cores; fp32 and other layouts on the FMA pipe (IEEE fp32).  At most 4096
+ * groups.  No counterpart in the reference, whose batched products
+ * (_cuda_ops.pyx:1122-1190) have one size for the whole batch. */
+int32_t sf_gemm_grouped(int64_t groups, int64_t M, int64_t N, int64_t K, const void* A,
+                        int64_t a_rows, int64_t lda, const int32_t* rows, const int32_t* offsets,
+                        const void* B, int64_t ldb, int64_t b_stride, const void* bias,
+                        int32_t bias_dtype, int64_t bias_stride, void* C, int64_t ldc,
+                        int32_t in_dtype, int32_t out_dtype, int32_t activation, void* stream);
+
+/* Router: the top_k experts of every token by logit (falling; ties to the
+ * lowest expert; NaN counts as -inf), their weights, and the choices grouped
+ * by expert for sf_gemm_grouped.
+ *   weights[t][j] = exp(z_j - z_0) / sum over the chosen (renormalize != 0)
+ *                   or over all experts (0); 0 for a chosen logit of -inf
+ *   slot p of offsets[e] <= p < offsets[e + 1] holds token rows[p], by rising
+ *   token; slots[t][j] is the slot of choice j of token t.
+ * expert_ids, weights and slots are [tokens][top_k], rows [tokens * top_k],
+ * offsets [experts + 1].  At most 1024 experts and top_k 32.  The same
+ * inputs give the same bits.  The workspace (0 bytes for few tokens) is free
+ * again when the call's kernels are done.  No counterpart in the reference. */
+int32_t sf_moe_route_workspace_size(int64_t tokens, int64_t experts, int32_t top_k, size_t* bytes);
+int32_t sf_moe_route(int64_t tokens, int64_t experts, int32_t top_k, const void* logits,
+                     int32_t dtype, int64_t ld, int32_t renormalize, int32_t* expert_ids,
+                     float* weights, int32_t* offsets, int32_t* rows, int32_t* slots,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[t, :] = residual[t, :] + sum_j weights[t][j] * y[slots[t][j], :] in
+ * fp32, rounded once (residual may be NULL; y, residual and out share dtype).
+ * A slot outside 0..y_rows-1 adds nothing.  out may be residual's memory, not
+ * y's.  No counterpart in the reference. */
+int32_t sf_moe_combine(int64_t tokens, int64_t cols, int32_t top_k, const void* y, int64_t y_rows,
+                       int64_t ldy, int32_t dtype, const int32_t* slots, const float* weights,
+                       const void* residual, int64_t ldr, void* out, int64_t ldo, void* stream);
+
+/* ───────────────────────── 4-bit weights ───────────────────────── */
+
+/* y[M,N] = act(x[M,K] . W[N,K]^T + bias) with
+ *   W[n, k] = scales[k / group, n] * (q[n, k] - zeros[k / group, n]),
+ * q in 0..15, zeros = 8 when NULL, for M <= 64 rows of bf16/fp16 x (the
+ * weights are read once).  scales and zeros are [ceil(K / group)][lds >= N]
+ * in x's type; group is 32, 64 or 128.  packed row n holds ldp >= 16 *
+ * ceil(K / 128) words (16-byte aligned, ldp a multiple of 4): nibble i (from
+ * the low end) of word 4 t + w of 128-column block b holds column
+ *   128 b + 32 w + 8 t + {0, 2, 4, 6, 1, 3, 5, 7}[i]
+ * (columns past K are ignored).  Sums in fp32.  Beside the skinny linears of
+ * sf_gemm; no counterpart in the reference. */
+int32_t sf_linear_w4(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
+                     const uint32_t* packed, int64_t ldp, const void* scales, const void* zeros,
+                     int64_t lds, int32_t group, const void* bias, int32_t bias_dtype, void* y,
+                     int64_t ldy, int32_t in_dtype, int32_t out_dtype, int32_t activation,
+                     void* stream);
+
+/* Quantises W [N,K] into that form.  zeros NULL: scale = max|w| / 7,
+ * q = rint(w / scale) + 8; else scale = (max - min) / 15 (0 counted in),
+ * zero = rint(-min / scale), q = rint(w / scale) + zero; the scale is rounded
+ * to scale_dtype before q is formed.  sf_dequantize_w4 writes W back in
+ * w_dtype, one rounding, for products with more rows. */
+int32_t sf_quantize_w4(int64_t N, int64_t K, const void* W, int32_t w_dtype, int64_t ldw,
+                       int32_t group, uint32_t* packed, int64_t ldp, void* scales, void* zeros,
+                       int64_t lds, int32_t scale_dtype, void* stream);
+int32_t sf_dequantize_w4(int64_t N, int64_t K, const uint32_t* packed, int64_t ldp,
+                         const void* scales, const void* zeros, int64_t lds, int32_t group,
+                         int32_t scale_dtype, void* W, int32_t w_dtype, int64_t ldw, void* stream);
 
 /* fp32 arithmetic mode (per process).  Replaces cuda_set_tf32
  * (_cuda_ops_decl.h:153, _cuda_kernels.cu:1928-1936). */

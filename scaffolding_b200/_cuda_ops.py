@@ -15,6 +15,9 @@ sm_100a engine (``libsf_engine.so``) instead of cuBLAS:
   ``dev_gelu``, ``dev_reshape``, ``dev_unsqueeze``, ``dev_squeeze``;
 * ``dev_layer_norm`` and the DiT blocks' adaptive norm ``dev_ada_layer_norm``
   (the bandwidth step in front of the QKV and FFN-up GEMMs);
+* the linears of a sparse language-model layer: ``dev_moe_route``,
+  ``dev_grouped_linear`` and ``dev_moe_combine``, and ``dev_linear_w4`` over
+  4-bit weights (``W4Weight``, ``dev_quantize_w4``, ``dev_dequantize_w4``);
 * runtime: devices, caching allocator, streams, events, peer access.
 
 Differences from the reference, all deliberate:
@@ -43,7 +46,7 @@ import math
 import numpy as np
 
 from . import engine as E
-from ._lib import (ACT_GELU_TANH, ACT_NONE, ACT_SILU, COPY_D2D, COPY_D2H, COPY_H2D,
+from ._lib import (ACT_GELU_TANH, ACT_NONE, ACT_SILU, ACT_SILU_GATE, COPY_D2D, COPY_D2H, COPY_H2D,
                    DT_F32, FP32_ACCURATE, FP32_TF32, DeviceProps, check, lib)
 
 bfloat16 = E.bfloat16
@@ -401,6 +404,321 @@ def dev_ada_layer_norm(gt: GpuTensor, gt_params: GpuTensor, gt_gamma: GpuTensor 
     if gt.ndim != 3 or gt_params.ndim != 2 or gt_params.shape[0] != gt.shape[0]:
         raise ValueError(f"adaLN shapes: x {gt.shape}, params {gt_params.shape}")
     return _norm_launch(gt, gt_gamma, gt_beta, eps, gt_params, gt.shape[1], out_dtype)
+
+
+# ───────────────────────────── experts ─────────────────────────────
+
+def _same_device(*tensors) -> int:
+    """Device of the tensors (None skipped); refuses a mix."""
+    devs = {t.device_id for t in tensors if t is not None}
+    if len(devs) != 1:
+        raise ValueError(f"operands on different devices ({' vs '.join(map(str, sorted(devs)))})")
+    return devs.pop()
+
+
+def _result(out, shape, dtype, dev, name: str) -> GpuTensor:
+    """``out`` when the caller gives the result's buffer, else a new tensor."""
+    if out is None:
+        return _alloc(shape, dtype, dev)
+    if out.shape != tuple(shape) or out.dtype != np.dtype(dtype):
+        raise ValueError(f"{name} must be {tuple(shape)} {np.dtype(dtype)}, got {out.shape} {out.dtype}")
+    return out
+
+
+def _int32(t: GpuTensor, name: str) -> GpuTensor:
+    if t.dtype != np.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    return t
+
+
+def _ptr(t):
+    return C.c_void_p(t.ptr) if t is not None else None
+
+
+def _stream_arg(dev: int):
+    s = E.get_stream(dev)
+    return C.c_void_p(s) if s else None
+
+
+class MoeRoute:
+    """A batch's choices of experts, as ``dev_moe_route`` gives them:
+
+    * ``experts`` int32 ``[tokens, top_k]``, by falling logit;
+    * ``weights`` fp32 ``[tokens, top_k]``;
+    * ``offsets`` int32 ``[experts + 1]``: the slots of expert e are
+      ``offsets[e] .. offsets[e + 1] - 1``;
+    * ``rows`` int32 ``[tokens * top_k]``: the token of each slot;
+    * ``slots`` int32 ``[tokens, top_k]``: the slot of each choice."""
+
+    __slots__ = ("experts", "weights", "offsets", "rows", "slots", "scratch")
+
+    def __init__(self, experts, weights, offsets, rows, slots):
+        self.experts, self.weights, self.offsets = experts, weights, offsets
+        self.rows, self.slots = rows, slots
+        self.scratch = None  # per-block counts, kept with the buffers they are used with
+
+
+def dev_moe_route(gt_logits: GpuTensor, top_k: int, renormalize: bool = True,
+                  out: MoeRoute | None = None) -> MoeRoute:
+    """Route ``[tokens, experts]`` logits (fp32 / bf16 / fp16): the ``top_k``
+    experts of every token (ties to the lowest expert, NaN as -inf), their
+    softmax weights -- over the chosen experts, or over all of them with
+    ``renormalize=False`` -- and the choices grouped by expert for
+    ``dev_grouped_linear`` (``sf_moe_route``).  ``out``: a MoeRoute whose
+    buffers are written instead of new ones (a captured graph, a decoding
+    loop); it must not be read by work in flight on another stream.  New (the
+    reference has no routed layers)."""
+    if gt_logits.ndim != 2:
+        raise ValueError(f"router logits must be [tokens, experts], got {gt_logits.shape}")
+    T, X = gt_logits.shape
+    k = int(top_k)
+    dev = gt_logits.device_id
+    code = E.dtype_code(gt_logits.dtype)
+    need = C.c_size_t()
+    check(lib.sf_moe_route_workspace_size(T, X, k, C.byref(need)), "sf_moe_route_workspace_size")
+    if out is None:
+        i32 = np.int32
+        out = MoeRoute(_alloc((T, k), i32, dev), _alloc((T, k), np.float32, dev),
+                       _alloc((X + 1,), i32, dev), _alloc((T * k,), i32, dev), _alloc((T, k), i32, dev))
+    else:
+        _same_device(gt_logits, out.experts, out.weights, out.offsets, out.rows, out.slots)
+        for name, shape in (("experts", (T, k)), ("weights", (T, k)), ("offsets", (X + 1,)),
+                            ("rows", (T * k,)), ("slots", (T, k))):
+            _result(getattr(out, name), shape, np.float32 if name == "weights" else np.int32, dev, name)
+    if need.value and (out.scratch is None or out.scratch.nbytes < need.value
+                       or out.scratch.device_id != dev):
+        out.scratch = _make_buffer(need.value, dev)
+    ws = C.c_void_p(out.scratch.ptr) if need.value else None
+    with E.on_device(dev):
+        check(lib.sf_moe_route(T, X, k, _ptr(gt_logits), code, X, 1 if renormalize else 0,
+                               _ptr(out.experts), _ptr(out.weights), _ptr(out.offsets),
+                               _ptr(out.rows), _ptr(out.slots), ws, need.value, _stream_arg(dev)),
+              "sf_moe_route")
+    return out
+
+
+def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTensor,
+                       gt_bias: GpuTensor | None = None, activation: str = "none", *,
+                       rows: GpuTensor | None = None, out_dtype=None,
+                       out: GpuTensor | None = None) -> GpuTensor:
+    """One linear per expert over rows grouped by expert, in one launch
+    (``sf_gemm_grouped``): output row i, ``offsets[e] <= i < offsets[e + 1]``,
+    is ``act(weight[e] @ x[r] + bias[e])`` with ``r = rows[i]`` when ``rows``
+    is given (the rows are gathered as they are read), else ``r = i``.
+
+    ``weight`` is ``[experts, N, K]``, each expert as an ``nn.Linear`` weight,
+    ``bias`` ``[experts, N]``.  ``activation="silu_gate"`` takes ``[experts,
+    2 N, K]``, the first N rows the gate: ``silu(gate) * value``.  The group
+    sizes stay on the device.  Rows of the result in no group are not written
+    (``dev_moe_route``'s offsets cover every row)."""
+    act = E.grouped_act_code(activation)
+    if gt_x.ndim != 2 or gt_weight.ndim != 3:
+        raise ValueError(f"grouped linear shapes: x {gt_x.shape}, weight {gt_weight.shape}")
+    if gt_x.dtype != gt_weight.dtype:
+        raise TypeError(f"matmul operands must share a dtype ({gt_x.dtype} vs {gt_weight.dtype})")
+    X, wide, K = gt_weight.shape
+    if gt_x.shape[1] != K:
+        raise ValueError(f"grouped linear shape mismatch: x {gt_x.shape}, weight {gt_weight.shape}")
+    if act == ACT_SILU_GATE and wide % 2:
+        raise ValueError(f"silu_gate needs gate and value rows, got {wide} rows per expert")
+    if _int32(gt_offsets, "offsets").shape != (X + 1,):
+        raise ValueError(f"offsets must be ({X + 1},), got {gt_offsets.shape}")
+    if rows is not None and _int32(rows, "rows").ndim != 1:
+        raise ValueError(f"rows must be 1-d, got {rows.shape}")
+    if gt_bias is not None and gt_bias.shape != (X, wide):
+        raise ValueError(f"bias must be {(X, wide)}, got {gt_bias.shape}")
+    N = wide // 2 if act == ACT_SILU_GATE else wide
+    M = rows.shape[0] if rows is not None else gt_x.shape[0]
+    dev = _same_device(gt_x, gt_weight, gt_offsets, gt_bias, rows, out)
+    odt = _out_dtype(gt_x, out_dtype if out is None else out.dtype)
+    y = _result(out, (M, N), odt, dev, "out")
+    bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
+    with E.on_device(dev):
+        check(lib.sf_gemm_grouped(X, M, N, K, _ptr(gt_x), gt_x.shape[0], K, _ptr(rows),
+                                  _ptr(gt_offsets), _ptr(gt_weight), K, wide * K, _ptr(gt_bias),
+                                  bias_dt, wide, _ptr(y), N, E.dtype_code(gt_x.dtype),
+                                  E.dtype_code(odt), act, _stream_arg(dev)), "sf_gemm_grouped")
+    return y
+
+
+def dev_moe_combine(gt_y: GpuTensor, gt_slots: GpuTensor, gt_weights: GpuTensor,
+                    residual: GpuTensor | None = None, out: GpuTensor | None = None) -> GpuTensor:
+    """Weighted sum of every token's expert rows (``sf_moe_combine``):
+    ``residual[t] + sum_j weights[t, j] * y[slots[t, j]]`` in fp32, rounded
+    once; ``slots`` and ``weights`` as in a MoeRoute, ``y`` ``[slots, C]``.
+    A slot outside ``y`` (-1, say, for a dropped choice) adds nothing."""
+    if gt_y.ndim != 2 or gt_slots.ndim != 2:
+        raise ValueError(f"combine shapes: y {gt_y.shape}, slots {gt_slots.shape}")
+    T, k = _int32(gt_slots, "slots").shape
+    width = gt_y.shape[1]
+    if gt_weights.shape != (T, k) or gt_weights.dtype != np.float32:
+        raise ValueError(f"weights must be {(T, k)} float32, got {gt_weights.shape} {gt_weights.dtype}")
+    if residual is not None and (residual.shape != (T, width) or residual.dtype != gt_y.dtype):
+        raise ValueError(f"residual must be {(T, width)} {gt_y.dtype}, got {residual.shape} {residual.dtype}")
+    dev = _same_device(gt_y, gt_slots, gt_weights, residual, out)
+    o = _result(out, (T, width), gt_y.dtype, dev, "out")
+    with E.on_device(dev):
+        check(lib.sf_moe_combine(T, width, k, _ptr(gt_y), gt_y.shape[0], width,
+                                 E.dtype_code(gt_y.dtype), _ptr(gt_slots), _ptr(gt_weights),
+                                 _ptr(residual), width, _ptr(o), width, _stream_arg(dev)),
+              "sf_moe_combine")
+    return o
+
+
+# ───────────────────────────── 4-bit weights ─────────────────────────────
+
+# Nibble i of a packed word holds column _W4_NIBBLE[i] of its eight.
+_W4_NIBBLE = (0, 2, 4, 6, 1, 3, 5, 7)
+_W4_MAX_ROWS = 64  # rows of x that sf_linear_w4 takes
+
+
+def pack_w4(q: np.ndarray) -> np.ndarray:
+    """Host ``[N, K]`` values 0..15 to ``[N, 16 * ceil(K / 128)]`` uint32
+    words in the order ``sf_linear_w4`` documents; columns past K hold 0."""
+    if q.ndim != 2 or (q.size and (q.min() < 0 or q.max() > 15)):
+        raise ValueError("4-bit values are a 2-d array of 0..15")
+    n, k = q.shape
+    blocks = -(-k // 128)
+    padded = np.zeros((n, blocks * 128), np.uint32)
+    padded[:, :k] = q
+    # [n, block, w, t, column of 8] -> words 4 t + w
+    cols = padded.reshape(n, blocks, 4, 4, 8).transpose(0, 1, 3, 2, 4)
+    words = np.zeros(cols.shape[:-1], np.uint32)
+    for i, c in enumerate(_W4_NIBBLE):
+        words |= cols[..., c] << np.uint32(4 * i)
+    return words.reshape(n, blocks * 16)
+
+
+class W4Weight:
+    """An ``[out_features, in_features]`` weight in 4 bits with group scales:
+    ``W[n, k] = scales[k // group, n] * (q[n, k] - zeros[k // group, n])``,
+    q in 0..15, zeros 8 where None.
+
+    * ``packed``: uint32 (or int32) ``[N, 16 * ceil(K / 128)]``, nibbles in
+      the order ``sf_linear_w4`` documents (``from_arrays`` packs);
+    * ``scales`` / ``zeros``: ``[ceil(K / group), N]`` in the type of the
+      activations (bf16 / fp16)."""
+
+    def __init__(self, packed: GpuTensor, scales: GpuTensor, zeros: GpuTensor | None = None, *,
+                 in_features: int, group: int = 128):
+        if group not in (32, 64, 128):
+            raise ValueError(f"group of {group} columns (32, 64 or 128)")
+        if packed.ndim != 2 or packed.dtype not in (np.dtype(np.uint32), np.dtype(np.int32)):
+            raise ValueError(f"packed must be 2-d uint32, got {packed.shape} {packed.dtype}")
+        n = packed.shape[0]
+        if packed.shape[1] != -(-in_features // 128) * 16:
+            raise ValueError(f"packed rows of {packed.shape[1]} words for {in_features} columns")
+        for t, name in ((scales, "scales"), (zeros, "zeros")):
+            if t is not None and t.shape != (-(-in_features // group), n):
+                raise ValueError(f"{name} must be {(-(-in_features // group), n)}, got {t.shape}")
+        if zeros is not None and zeros.dtype != scales.dtype:
+            raise TypeError(f"scales and zeros must share a dtype ({scales.dtype} vs {zeros.dtype})")
+        _same_device(packed, scales, zeros)
+        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self.in_features, self.out_features, self.group = int(in_features), n, int(group)
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return (self.out_features, self.in_features)
+
+    @property
+    def device_id(self) -> int:
+        return self.packed.device_id
+
+    @classmethod
+    def from_arrays(cls, q: np.ndarray, scales: np.ndarray, zeros: np.ndarray | None = None,
+                    group: int = 128, device_id: int = -1) -> "W4Weight":
+        """From host arrays as checkpoints hold them: ``q [N, K]`` in 0..15,
+        ``scales`` and ``zeros`` ``[N, ceil(K / group)]``; packed on the host."""
+        n, k = q.shape
+        up = lambda a: gputensor_from_numpy(np.ascontiguousarray(a), device_id)  # noqa: E731
+        return cls(up(pack_w4(q)), up(scales.T),
+                   up(zeros.T) if zeros is not None else None, in_features=k, group=group)
+
+    def to(self, target_dev: int) -> "W4Weight":
+        """Copy on another device."""
+        if self.device_id == target_dev:
+            return self
+        move = lambda t: gputensor_to_device(t, target_dev) if t is not None else None  # noqa: E731
+        return W4Weight(move(self.packed), move(self.scales), move(self.zeros),
+                        in_features=self.in_features, group=self.group)
+
+
+def dev_quantize_w4(gt_weight: GpuTensor, group: int = 128, zeros: bool = False,
+                    dtype=None) -> W4Weight:
+    """Quantise an ``[N, K]`` weight to 4 bits on its device
+    (``sf_quantize_w4``): scale max|w| / 7 around 8, or, with ``zeros``, scale
+    and zero point of each group's range.  ``dtype``: type of the scales,
+    that of the activations the weight will meet (default: the weight's)."""
+    if gt_weight.ndim != 2:
+        raise ValueError(f"weight must be [N, K], got {gt_weight.shape}")
+    if group not in (32, 64, 128):
+        raise ValueError(f"group of {group} columns (32, 64 or 128)")
+    n, k = gt_weight.shape
+    dev = gt_weight.device_id
+    sdt = np.dtype(dtype) if dtype is not None else gt_weight.dtype
+    words, groups = -(-k // 128) * 16, -(-k // group)
+    packed = _alloc((n, words), np.uint32, dev)
+    scales = _alloc((groups, n), sdt, dev)
+    zs = _alloc((groups, n), sdt, dev) if zeros else None
+    with E.on_device(dev):
+        check(lib.sf_quantize_w4(n, k, _ptr(gt_weight), E.dtype_code(gt_weight.dtype), k, group,
+                                 _ptr(packed), words, _ptr(scales), _ptr(zs), n,
+                                 E.dtype_code(sdt), _stream_arg(dev)), "sf_quantize_w4")
+    return W4Weight(packed, scales, zs, in_features=k, group=group)
+
+
+def dev_dequantize_w4(weight: W4Weight, dtype=None) -> GpuTensor:
+    """The ``[N, K]`` weight a W4Weight stands for, in ``dtype`` (default: its
+    scales' type), each value rounded once."""
+    n, k = weight.shape
+    dev = weight.device_id
+    wdt = np.dtype(dtype) if dtype is not None else weight.scales.dtype
+    w = _alloc((n, k), wdt, dev)
+    with E.on_device(dev):
+        check(lib.sf_dequantize_w4(n, k, _ptr(weight.packed), weight.packed.shape[1],
+                                   _ptr(weight.scales), _ptr(weight.zeros), n, weight.group,
+                                   E.dtype_code(weight.scales.dtype), _ptr(w), E.dtype_code(wdt), k,
+                                   _stream_arg(dev)), "sf_dequantize_w4")
+    return w
+
+
+def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None = None,
+                  activation: str = "none", out_dtype=None, out: GpuTensor | None = None) -> GpuTensor:
+    """``dev_linear_forward`` over a 4-bit weight: ``act(x @ W^T + bias)`` for
+    bf16 / fp16 x.  Up to 64 rows of x run on ``sf_linear_w4``, which streams
+    the packed weight once; more rows dequantise it into a 16-bit weight (one
+    more rounding per weight, which the streamed product does not make) and
+    run the GEMM."""
+    act = E.act_code(activation)
+    if gt_x.dtype != weight.scales.dtype:
+        raise TypeError(f"x and the weight's scales must share a dtype ({gt_x.dtype} vs {weight.scales.dtype})")
+    if gt_x.dtype == np.float32:
+        raise TypeError("4-bit linears take bf16 or fp16 x")
+    n, k = weight.shape
+    if gt_x.ndim < 1 or gt_x.shape[-1] != k:
+        raise ValueError(f"linear shape mismatch: x {gt_x.shape}, W {weight.shape}")
+    if gt_bias is not None and gt_bias.numel != n:
+        raise ValueError(f"bias has {gt_bias.numel} elements, expected {n}")
+    M = int(math.prod(gt_x.shape[:-1]))
+    dev = _same_device(gt_x, weight.packed, gt_bias, out)
+    odt = _out_dtype(gt_x, out_dtype if out is None else out.dtype)
+    y = _result(out, gt_x.shape[:-1] + (n,), odt, dev, "out")
+    bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
+    in_code, out_code = E.dtype_code(gt_x.dtype), E.dtype_code(odt)
+    with E.on_device(dev):
+        if M <= _W4_MAX_ROWS:
+            check(lib.sf_linear_w4(M, n, k, _ptr(gt_x), k, _ptr(weight.packed),
+                                   weight.packed.shape[1], _ptr(weight.scales), _ptr(weight.zeros),
+                                   n, weight.group, _ptr(gt_bias), bias_dt, _ptr(y), n, in_code,
+                                   out_code, act, _stream_arg(dev)), "sf_linear_w4")
+        else:
+            w = dev_dequantize_w4(weight)
+            epi = E.make_epilogue(bias_ptr=gt_bias.ptr if gt_bias is not None else 0,
+                                  bias_dt=bias_dt, act=act)
+            E.gemm(M, n, k, gt_x.ptr, k, 0, w.ptr, k, 1, y.ptr, n, in_code, out_code, epi=epi,
+                   device=dev)
+    return y
 
 
 def dev_unsqueeze(gt: GpuTensor, dim: int) -> GpuTensor:

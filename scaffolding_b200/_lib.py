@@ -25,6 +25,7 @@ SF_ERR_NCCL = -7
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 ACT_NONE, ACT_SILU, ACT_GELU_TANH = 0, 1, 2
+ACT_SILU_GATE = 3  # sf_gemm_grouped only
 FP32_ACCURATE, FP32_FFMA, FP32_TF32 = 0, 1, 2
 KERNEL_AUTO, KERNEL_TCGEN05, KERNEL_SIMT = 0, 1, 2
 COPY_H2D, COPY_D2H, COPY_D2D, COPY_DEFAULT = 0, 1, 2, 3
@@ -73,6 +74,17 @@ SIGNATURES: dict[str, list] = {
     "sf_linear_skinny_noalloc": [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i64,
                                  _i32, _i32, _i32, _vp],
     "sf_gemm_workspace_size": [_P(Batch), _i64, _i64, _i64, _i32, _i32, _i32, _i32, _P(_sz)],
+    "sf_gemm_grouped": [_i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
+                        _i32, _i64, _vp, _i64, _i32, _i32, _i32, _vp],
+    "sf_moe_route_workspace_size": [_i64, _i64, _i32, _P(_sz)],
+    "sf_moe_route": [_i64, _i64, _i32, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                     _vp],
+    "sf_moe_combine": [_i64, _i64, _i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _i64, _vp, _i64,
+                       _vp],
+    "sf_linear_w4": [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _vp,
+                     _i64, _i32, _i32, _i32, _vp],
+    "sf_quantize_w4": [_i64, _i64, _vp, _i32, _i64, _i32, _vp, _i64, _vp, _vp, _i64, _i32, _vp],
+    "sf_dequantize_w4": [_i64, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _i32, _i64, _vp],
     "sf_set_fp32_mode": [_i32],
     "sf_get_fp32_mode": [_P(_i32)],
     "sf_set_kernel_override": [_i32],

@@ -24,7 +24,7 @@ BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libsf_engine.so")
 
 SOURCES = ["runtime.cu", "engine.cu", "attention.cu", "norm.cu", "noalloc.cu", "peer.cu",
-           "comm.cpp"]
+           "moe.cu", "grouped.cu", "w4.cu", "comm.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -13,7 +13,7 @@ import threading
 import numpy as np
 
 from . import _lib
-from ._lib import (ACT_GELU_TANH, ACT_NONE, ACT_SILU, DT_BF16, DT_F16, DT_F32, Batch,
+from ._lib import (ACT_GELU_TANH, ACT_NONE, ACT_SILU, ACT_SILU_GATE, DT_BF16, DT_F16, DT_F32, Batch,
                    Epilogue, check, lib)
 
 try:  # bf16 host storage (NumPy has none; the reference maps bf16 to fp32, dtype.py:31)
@@ -24,6 +24,7 @@ except ImportError:  # pragma: no cover - ml_dtypes ships with this image
 
 _ACTS = {"none": ACT_NONE, None: ACT_NONE, "silu": ACT_SILU, "gelu_tanh": ACT_GELU_TANH,
          "gelu": ACT_GELU_TANH}
+_GROUPED_ACTS = {**_ACTS, "silu_gate": ACT_SILU_GATE}
 
 
 def dtype_code(dtype) -> int:
@@ -46,6 +47,14 @@ def act_code(act) -> int:
         return _ACTS[act]
     except KeyError:
         raise ValueError(f"unknown activation {act!r} (none | silu | gelu_tanh)") from None
+
+
+def grouped_act_code(act) -> int:
+    """Activation of a grouped product: those of act_code and ``silu_gate``."""
+    try:
+        return _GROUPED_ACTS[act]
+    except KeyError:
+        raise ValueError(f"unknown activation {act!r} (none | silu | gelu_tanh | silu_gate)") from None
 
 
 # ───────────────────────────── devices ─────────────────────────────

@@ -17,6 +17,9 @@ argument meaning and error behaviour:
   (one batched launch, scale fused in its epilogue), row softmax, P.V.
 * ``functional.silu`` / ``gelu`` / ``softmax`` -- ``nn/functional.py:37-145``.
 * ``Sequential`` -- the container the reference's models stack layers in.
+* ``Linear4`` -- ``Linear`` over a weight in 4 bits with group scales, and
+  ``MoE`` -- a routed feed-forward layer of expert linears (both new: the
+  sparse layers of language models, next to the dense ones).
 * ``LayerNorm`` (``nn/layers.py:443-521``) and ``AdaLayerNorm``
   (``diffusion/models.py:470-487``), the norms in front of the DiT linears.
 """
@@ -92,6 +95,103 @@ class Linear:
         self._to(x.device_id)
         ops.set_device(x.device_id)
         return ops.dev_linear_forward(x, self.weight, self.bias, activation)
+
+    __call__ = forward
+
+
+class Linear4:
+    """y = act(x W^T + b) with W in 4 bits (``ops.W4Weight``); x and the bias
+    in bf16 or fp16, the type of the weight's scales."""
+
+    def __init__(self, weight: ops.W4Weight, bias: GpuTensor | None = None):
+        self.weight = weight
+        self.bias = bias
+        self.out_features, self.in_features = weight.shape
+
+    @classmethod
+    def from_linear(cls, linear: Linear, group: int = 128, zeros: bool = False,
+                    dtype=None) -> "Linear4":
+        """Quantise a Linear on its device.  ``dtype``: bf16 or fp16, needed
+        when the Linear holds fp32."""
+        dt = np.dtype(dtype) if dtype is not None else linear.weight.dtype
+        bias = ops.gputensor_astype(linear.bias, dt) if linear.bias is not None else None
+        return cls(ops.dev_quantize_w4(linear.weight, group, zeros, dt), bias)
+
+    def to(self, device=None, dtype=None) -> "Linear4":
+        """Move to ``device``; the packed weight has no other dtype."""
+        if dtype is not None and np.dtype(dtype) != self.weight.scales.dtype:
+            raise TypeError(f"a 4-bit weight for {self.weight.scales.dtype} is not converted to {np.dtype(dtype)}")
+        if device is not None:
+            self._to(_device_index(device))
+        return self
+
+    def _to(self, dev: int) -> None:
+        self.weight = self.weight.to(dev)
+        if self.bias is not None and self.bias.device_id != dev:
+            self.bias = ops.gputensor_to_device(self.bias, dev)
+
+    def forward(self, x: GpuTensor, activation: str = "none") -> GpuTensor:
+        self._to(x.device_id)
+        return ops.dev_linear_w4(x, self.weight, self.bias, activation)
+
+    __call__ = forward
+
+
+class MoE:
+    """Routed feed-forward layer: every token goes through ``top_k`` of
+    ``num_experts`` two-layer experts, weighted by the router,
+
+        y = sum_j w_j down[e_j] act(up[e_j] x)     (+ residual)
+
+    router ``[experts, dim]``, ``up`` ``[experts, hidden, dim]`` (``[experts,
+    2 hidden, dim]`` for ``silu_gate``), ``down`` ``[experts, dim, hidden]``,
+    all drawn like Linear's weights.  Five launches for a decoding batch, six
+    for a prompt; the group sizes never leave the device."""
+
+    def __init__(self, dim: int, hidden: int, num_experts: int, top_k: int = 2,
+                 activation: str = "silu_gate", renormalize: bool = True, device=None,
+                 dtype=np.float32, rng: np.random.Generator | None = None):
+        if not 1 <= top_k <= num_experts:
+            raise ValueError(f"top_k {top_k} of {num_experts} experts")
+        self.dim, self.hidden = dim, hidden
+        self.num_experts, self.top_k = num_experts, top_k
+        self.activation, self.renormalize = activation, renormalize
+        gate = E.grouped_act_code(activation) == E.ACT_SILU_GATE
+        dev = _device_index(device)
+        gen = rng if rng is not None else np.random
+
+        def draw(fan_in, *shape):
+            k = 1.0 / math.sqrt(fan_in)
+            w = gen.uniform(-k, k, shape).astype(np.float32).astype(dtype)
+            return ops.gputensor_from_numpy(w, dev)
+
+        self.router = draw(dim, num_experts, dim)
+        self.up = draw(dim, num_experts, hidden * (2 if gate else 1), dim)
+        self.down = draw(hidden, num_experts, dim, hidden)
+
+    def to(self, device=None, dtype=None) -> "MoE":
+        for name in ("router", "up", "down"):
+            w = getattr(self, name)
+            if device is not None:
+                w = ops.gputensor_to_device(w, _device_index(device))
+            setattr(self, name, ops.gputensor_astype(w, dtype) if dtype is not None else w)
+        return self
+
+    def forward(self, x: GpuTensor, residual: GpuTensor | None = None) -> GpuTensor:
+        """``x [..., dim]`` to the same shape; ``residual`` (that shape too)
+        is added to the experts' sum before it is rounded."""
+        if self.router.device_id != x.device_id:
+            self.to(x.device_id)
+        if residual is not None and residual.shape != x.shape:
+            raise ValueError(f"residual must be {x.shape}, got {residual.shape}")
+        flat = ops.dev_reshape(x, (x.numel // self.dim, self.dim))
+        logits = ops.dev_linear_forward(flat, self.router, out_dtype=np.float32)
+        route = ops.dev_moe_route(logits, self.top_k, self.renormalize)
+        h = ops.dev_grouped_linear(flat, self.up, route.offsets, activation=self.activation,
+                                   rows=route.rows)
+        y = ops.dev_grouped_linear(h, self.down, route.offsets)
+        res = ops.dev_reshape(residual, flat.shape) if residual is not None else None
+        return ops.dev_reshape(ops.dev_moe_combine(y, route.slots, route.weights, res), x.shape)
 
     __call__ = forward
 
