@@ -3,9 +3,10 @@
 //   y[m, n] = act(sum_k x[m, k] W[n, k] + bias[n]),
 //   W[n, k] = scale[k / g, n] * (q[n, k] - zero[k / g, n]),  q in 0..15,
 //
-// zero = 8 where none is stored.  q, zero (an integer in practice) and their
-// difference are exact in 16 bits, the scale stays out of the products: a
-// group's sum of x * (q - zero) is formed in fp32 and scaled once.
+// zero = 8 where none is stored, else the whole number in 0..15 nearest to the
+// stored value.  q, zero and their difference are exact in 16 bits, the scale
+// stays out of the products: a group's sum of x * (q - zero) is formed in fp32
+// and scaled once.
 //
 // Layout of q: row n is a run of 32-bit words, 16 per block of 128 columns
 // (K is padded to whole blocks; what the padding holds is not used).  Nibble i
@@ -18,6 +19,7 @@
 
 #include "common.h"
 #include "epilogue.cuh"
+#include "ptx.cuh"
 #include "tma_host.h"
 
 namespace sf {
@@ -50,36 +52,338 @@ __host__ __device__ __forceinline__ int w4_column(int j, int i) {
   return 32 * (j & 3) + 8 * (j >> 2) + (i < 4 ? 2 * i : 2 * i - 7);
 }
 
-// One warp per output row n, eight rows of x at a time.
-__global__ void __launch_bounds__(256) w4_linear_kernel(const W4Args a) {
-  const int lane = threadIdx.x & 31;
-  const int n = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  if (n >= a.N) return;
-  const int words = static_cast<int>((a.K + 127) / 128 * 16);
-  for (int m0 = 0; m0 < a.M; m0 += 8) {
-    float acc[8] = {};
-    for (int wd = lane; wd < words; wd += 32) {
-      const uint32_t q = a.packed[n * a.ldp + wd];
-      const int base = wd / 16 * 128;
-      for (int i = 0; i < 8; ++i) {
-        const int k = base + w4_column(wd & 15, i);
-        if (k >= a.K) continue;
-        const int64_t at = static_cast<int64_t>(k / a.group) * a.lds + n;
-        const float z = a.zeros ? load_as_f32(a.zeros, at, a.dtype) : 8.0f;
-        const float w = load_as_f32(a.scales, at, a.dtype) * (static_cast<float>((q >> (4 * i)) & 15u) - z);
-        for (int m = 0; m < 8; ++m)
-          if (m0 + m < a.M) acc[m] = fmaf(w, load_as_f32(a.x, (m0 + m) * a.ldx + k, a.dtype), acc[m]);
-      }
+// ───────────────────────── up to 64 rows of x ─────────────────────────
+// Weights as the 16-row side of mma.m16n8k16, rows of x as its 8 columns: the
+// product is bound by the weight stream (half a byte per weight against 16
+// multiply-adds at most 8 rows), and what has to keep up with it is the
+// unpacking.  At 6.5 TB/s a lane has 2.8 issue slots per weight.  A packed
+// word becomes four operand registers by masking two nibbles at a time into
+// the mantissas of 128 (bf16) or 1024 (fp16) and subtracting that plus the
+// zero point, which is exact: 1.1 to 1.4 operations per weight, one scale and
+// four multiply-adds per group, and the tensor core does the products.
+//
+// A warp owns 32 weight rows and every WK-th 128-column block of them.  In a
+// block, lane (g, t) = (lane / 4, lane % 4) takes 16 bytes of each of rows g,
+// g + 8, g + 16, g + 24: words 4 t .. 4 t + 3, whose columns 32 w + 8 t .. + 7
+// are one 16-byte piece of x for token g.  The order of k within an mma is free
+// as long as both operands agree, so the layout makes every copy of both
+// operands 16 bytes and word w of all four t one 32-column group.  Words and x
+// travel through a ring of asynchronous copies; scales are loaded two blocks
+// ahead, one row per lane.  The WK partial sums of a row meet in shared memory,
+// in warp order.  More than 16 rows of x run in passes of 16.
+
+constexpr int kW4Threads = 256;
+constexpr int kW4Rows = 32;   // weight rows of a warp
+constexpr int kW4Stages = 3;  // blocks in flight per warp
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// (v & mask) | magic as the one logic operation that it is.
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(magic));
+  return r;
+}
+
+// A stored zero point as the whole number 0..15 it stands for.
+__device__ __forceinline__ float whole_zero(float z) { return fminf(fmaxf(rintf(z), 0.0f), 15.0f); }
+
+// Word -> four pairs (columns 2 i, 2 i + 1) of q - z.  z is the pair constant
+// of the group: 128 + z (bf16); 1024 + z in .x and 64 + z in .y (fp16).
+template <bool BF16>
+__device__ __forceinline__ void unpack_word(uint32_t w, uint2 z, uint32_t (&p)[4]) {
+  if constexpr (BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&z.x));
+      p[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
-    for (int m = 0; m < 8; ++m) {
-      for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
-      if (lane == 0 && m0 + m < a.M) {
-        float v = acc[m] + (a.bias ? load_as_f32(a.bias, n, a.bias_dtype) : 0.0f);
-        v = a.fast_act ? act_apply_fast(v, a.act) : act_apply(v, a.act);
-        store_from_f32(a.y, (m0 + m) * a.ldy + n, a.out_dtype, v);
+  } else {
+    const uint32_t sixteenth = 0x2C002C00u;  // 1/16, 1/16
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t u = h ? w >> 8 : w;
+      const uint32_t lo = and_or(u, 0x000F000Fu, 0x64006400u);  // 1024 + q
+      const uint32_t hi = and_or(u, 0x00F000F0u, 0x64006400u);  // 1024 + 16 q
+      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&z.x));
+      const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi),
+                                *reinterpret_cast<const __half2*>(&sixteenth),
+                                __hneg2(*reinterpret_cast<const __half2*>(&z.y)));
+      p[2 * h] = *reinterpret_cast<const uint32_t*>(&a);
+      p[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+}
+
+// The pair constant of a stored zero point (16 bits, low half of v): adding
+// the magic rounds it to a whole number, the clamp keeps it in 0..15 (a NaN
+// becomes 0), as whole_zero does.
+template <bool BF16>
+__device__ __forceinline__ uint2 zero_pair(uint16_t v) {
+  const uint32_t two = static_cast<uint32_t>(v) * 0x10001u;
+  uint2 r;
+  if constexpr (BF16) {
+    __nv_bfloat162 m = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&two), __float2bfloat162_rn(128.0f));
+    m = __hmin2(__hmax2(m, __float2bfloat162_rn(128.0f)), __float2bfloat162_rn(143.0f));
+    r.x = *reinterpret_cast<const uint32_t*>(&m);
+    r.y = 0;
+  } else {
+    __half2 m = __hadd2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(1024.0f));
+    m = __hmin2(__hmax2(m, __float2half2_rn(1024.0f)), __float2half2_rn(1039.0f));
+    const __half2 n = __hsub2(m, __float2half2_rn(960.0f));
+    r.x = *reinterpret_cast<const uint32_t*>(&m);
+    r.y = *reinterpret_cast<const uint32_t*>(&n);
+  }
+  return r;
+}
+
+// Eight columns of x at p, of which `left` lie before K; 0 past them.
+__device__ __forceinline__ uint4 load_x8_ragged(const uint16_t* p, int left) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) w[i >> 1] |= static_cast<uint32_t>(p[i]) << (16 * (i & 1));
+  return v;
+}
+
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Zeros instead of the 16 bytes when !in (nothing is read then).
+__device__ __forceinline__ void copy_async16_if(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// GW: 32-column words per group (1, 2, 4).
+template <bool BF16, int NT, int GW>
+__global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int wk, int x_vec) {
+  constexpr int NG = 4 / GW;             // groups per block
+  constexpr int kSlot = (4 + 4 * NT) * 32;  // 16-byte vectors per block: a lane's words and x
+  // Each lane's own words and x, kW4Stages blocks ahead: a lane reads back only
+  // what it copied itself, so its own wait on the copies is all the order needed.
+  extern __shared__ __align__(16) uint8_t sm[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int kw = warp % wk, per_cta = (blockDim.x >> 5) / wk;
+  const int n0 = (blockIdx.x * per_cta + warp / wk) * kW4Rows;
+  const int blocks = (a.K + 127) / 128, groups = (a.K + 32 * GW - 1) / (32 * GW);
+  const int mine = n0 < a.N ? (blocks - kw + wk - 1) / wk : 0;  // blocks kw, kw + wk, ...
+  uint4* const ring = reinterpret_cast<uint4*>(sm) + warp * (kW4Stages * kSlot) + lane;
+  const uint32_t ring_s = smem_u32(ring);
+
+  float acc[2][NT][4] = {};
+  // rows past N read row N - 1 and are not stored; tokens past M are not
+  // copied (their columns of the products are not stored either)
+  const uint4* src[4];  // rows n0 + 8 j + g
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    src[j] = reinterpret_cast<const uint4*>(a.packed + min(n0 + 8 * j + g, a.N - 1) * a.ldp) + t + 4 * kw;
+  const uint16_t* xp = static_cast<const uint16_t*>(a.x) + g * a.ldx + 128 * kw + 8 * t;
+  int left = a.K - (128 * kw + 8 * t);  // columns from xp to the row's end
+  // scales and zeros of row n0 + lane, shared out by shuffles
+  const uint16_t* sp = static_cast<const uint16_t*>(a.scales) + kw * NG * a.lds + min(n0 + lane, a.N - 1);
+  const uint16_t* zp = static_cast<const uint16_t*>(a.zeros) + kw * NG * a.lds + min(n0 + lane, a.N - 1);
+  const int64_t s_step = static_cast<int64_t>(wk) * NG * a.lds;
+  const bool zeros = a.zeros != nullptr;
+
+  int copied = 0;
+  auto copy_block = [&](int slot) {
+    if (copied < mine) {
+      const uint32_t dst = ring_s + slot * kSlot * 16;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        copy_async16(dst + j * 32 * 16, src[j]);
+        src[j] += 4 * wk;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (8 * n + g < a.M) {
+          const uint16_t* p = xp + 8 * n * a.ldx;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if (x_vec)
+              copy_async16_if(dst + (4 + 4 * n + w) * 32 * 16, 32 * w < left ? p + 32 * w : p, 32 * w < left);
+            else
+              ring[slot * kSlot + (4 + 4 * n + w) * 32] = load_x8_ragged(p + 32 * w, left - 32 * w);
+          }
+        }
+      xp += 128 * wk;
+      left -= 128 * wk;
+    }
+    ++copied;
+    copy_async_commit();
+  };
+  int scaled = 0;
+  uint16_t sc[3][NG], ze[3][NG];  // two blocks ahead
+  auto load_scales = [&](int to) {
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const bool in = scaled < mine && (kw + scaled * wk) * NG + j < groups;
+      sc[to][j] = in ? __ldg(sp + j * a.lds) : 0;
+      ze[to][j] = in && zeros ? __ldg(zp + j * a.lds) : 0;
+    }
+    ++scaled;
+    sp += s_step;
+    zp += s_step;
+  };
+  auto as_float = [](uint16_t v) {
+    return BF16 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v));
+  };
+  load_scales(0);
+  load_scales(1);
+  for (int i = 0; i < kW4Stages - 1; ++i) copy_block(i);
+#pragma unroll 1
+  for (int i0 = 0; i0 < mine; i0 += kW4Stages) {
+#pragma unroll
+    for (int u = 0; u < kW4Stages; ++u) {
+      if (i0 + u >= mine) break;
+      copy_block((u + kW4Stages - 1) % kW4Stages);
+      float sv[NG];
+      uint2 zv[NG];
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        sv[j] = as_float(sc[u][j]);
+        if (zeros) zv[j] = zero_pair<BF16>(ze[u][j]);
+      }
+      load_scales((u + 2) % 3);
+      copy_async_wait<kW4Stages - 1>();
+      uint4 q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = ring[u * kSlot + j * 32];
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        float s[4];
+        uint2 z[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[r] = __shfl_sync(0xffffffffu, sv[j], 8 * r + g);
+          z[r] = make_uint2(BF16 ? 0x43084308u : 0x64086408u, 0x54805480u);  // + 8
+          if (zeros) {
+            z[r].x = __shfl_sync(0xffffffffu, zv[j].x, 8 * r + g);
+            if constexpr (!BF16) z[r].y = __shfl_sync(0xffffffffu, zv[j].y, 8 * r + g);
+          }
+        }
+        float sum[2][NT][4] = {};
+#pragma unroll
+        for (int l = 0; l < GW; ++l) {
+          const int w = j * GW + l;
+          uint32_t p[4][4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            unpack_word<BF16>(w == 0 ? q[r].x : w == 1 ? q[r].y : w == 2 ? q[r].z : q[r].w, z[r], p[r]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 x = ring[u * kSlot + (4 + 4 * n + w) * 32];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t a0[4] = {p[2 * r][0], p[2 * r + 1][0], p[2 * r][1], p[2 * r + 1][1]};
+              const uint32_t a1[4] = {p[2 * r][2], p[2 * r + 1][2], p[2 * r][3], p[2 * r + 1][3]};
+              mma_16816<BF16>(sum[r][n], a0, x.x, x.y);
+              mma_16816<BF16>(sum[r][n], a1, x.z, x.w);
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              acc[r][n][c] = fmaf(s[2 * r + (c >> 1)], sum[r][n][c], acc[r][n][c]);
       }
     }
   }
+  copy_async_wait<0>();
+  __syncthreads();  // every warp is done with its ring: the sums take its place
+  // [token][row] of this warp: acc c is row g + 8 (c / 2), token 2 t + c % 2
+  float* const red = reinterpret_cast<float*>(sm);
+  float* const part = red + warp * kW4Rows * (8 * NT);
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        part[(8 * n + 2 * t + (c & 1)) * kW4Rows + 16 * r + g + 8 * (c >> 1)] = acc[r][n][c];
+  __syncthreads();
+  // token-major: consecutive threads store consecutive columns of y
+  const int per_tile = kW4Rows * a.M;
+  for (int i = threadIdx.x; i < per_tile * per_cta; i += blockDim.x) {
+    const int tl = i / per_tile, e = i - tl * per_tile;
+    const int m = e / kW4Rows, r = e % kW4Rows;
+    const int n = (blockIdx.x * per_cta + tl) * kW4Rows + r;
+    if (n >= a.N) continue;
+    float v = 0.0f;
+    for (int w = 0; w < wk; ++w) v += red[(tl * wk + w) * kW4Rows * (8 * NT) + e];
+    if (a.bias) v += load_as_f32(a.bias, n, a.bias_dtype);
+    v = a.fast_act ? act_apply_fast(v, a.act) : act_apply(v, a.act);
+    store_from_f32(a.y, m * a.ldy + n, a.out_dtype, v);
+  }
+}
+
+template <bool BF16, int NT, int GW>
+int32_t launch_w4(const W4Args& a, bool x_vec, cudaStream_t s) {
+  // Warps along k: as many as there are blocks for, so that every row's
+  // stream is spread over the CTA; the rest take further rows.
+  const int64_t blocks = ceil_div(a.K, 128);
+  constexpr int warps = kW4Threads / 32;
+  int wk = 1;
+  while (wk < warps && wk < blocks) wk *= 2;
+  const int64_t rows = kW4Rows * (warps / wk);
+  const size_t smem = static_cast<size_t>(warps) *
+                      std::max(kW4Stages * (4 + 4 * NT) * 32 * 16, kW4Rows * 8 * NT * static_cast<int>(sizeof(float)));
+  SF_CUDA_TRY(cudaFuncSetAttribute(w4_mma_kernel<BF16, NT, GW>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  w4_mma_kernel<BF16, NT, GW>
+      <<<static_cast<unsigned>(ceil_div(a.N, rows)), warps * 32, smem, s>>>(a, wk, x_vec ? 1 : 0);
+  SF_CUDA_TRY(cudaGetLastError());
+  return SF_OK;
+}
+
+template <bool BF16, int NT>
+int32_t launch_w4_group(const W4Args& a, bool x_vec, cudaStream_t s) {
+  if (a.group == 32) return launch_w4<BF16, NT, 1>(a, x_vec, s);
+  if (a.group == 64) return launch_w4<BF16, NT, 2>(a, x_vec, s);
+  return launch_w4<BF16, NT, 4>(a, x_vec, s);
+}
+
+template <bool BF16>
+int32_t run_w4(const W4Args& a, cudaStream_t s) {
+  const bool x_vec = a.K % 8 == 0 && a.ldx % 8 == 0 && aligned16(a.x);
+  if (a.M <= 8) return launch_w4_group<BF16, 1>(a, x_vec, s);
+  W4Args p = a;
+  for (int m0 = 0; m0 < a.M; m0 += 16) {
+    p.M = std::min(16, a.M - m0);
+    p.x = static_cast<const uint16_t*>(a.x) + m0 * a.ldx;
+    p.y = static_cast<char*>(a.y) + m0 * a.ldy * esize(a.out_dtype);
+    const int32_t st = launch_w4_group<BF16, 2>(p, x_vec, s);
+    if (st != SF_OK) return st;
+  }
+  return SF_OK;
 }
 
 // Quantisation of one group of one row per warp-quarter is not worth a tuned
@@ -140,7 +444,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(int N, int K, const 
       const int k = base + w4_column(wd & 15, j);
       if (k >= K) continue;
       const int64_t at = static_cast<int64_t>(k / group) * lds + n;
-      const float z = zeros ? load_as_f32(zeros, at, s_dtype) : 8.0f;
+      const float z = zeros ? whole_zero(load_as_f32(zeros, at, s_dtype)) : 8.0f;
       store_from_f32(W, n * ldw + k, w_dtype,
                      load_as_f32(scales, at, s_dtype) * (static_cast<float>((q >> (4 * j)) & 15u) - z));
     }
@@ -196,9 +500,8 @@ int32_t sf_linear_w4(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx
   const W4Args a{static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), x, ldx, packed, ldp,
                  scales, zeros, lds, group, in_dtype, bias, bias_dtype, y, ldy, out_dtype, activation,
                  out_dtype != kF32 ? 1 : 0};
-  w4_linear_kernel<<<static_cast<unsigned>(ceil_div(N, 8)), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  SF_CUDA_TRY(cudaGetLastError());
-  return SF_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return in_dtype == kBF16 ? run_w4<true>(a, s) : run_w4<false>(a, s);
 }
 
 int32_t sf_quantize_w4(int64_t N, int64_t K, const void* W, int32_t w_dtype, int64_t ldw,
