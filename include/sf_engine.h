@@ -166,7 +166,7 @@ int32_t sf_linear_skinny_noalloc(int64_t M, int64_t N, int64_t K,
  * (device, [M], in 0..a_rows-1) are not read by the host: one launch whatever
  * the group sizes are, empty groups included.  Row i of C that lies in no
  * group is not written; an index outside 0..a_rows-1 reads a row of zeros;
- * offsets outside 0..M are clamped.
+ * offsets are clamped to 0..M and to their running maximum.
  *   B [groups][N][K] in the nn.Linear layout ([groups][2 N][K] for
  *   SF_ACT_SILU_GATE: N gate rows, then N value rows), rows ldb apart and
  *   groups b_stride apart; bias likewise, bias_stride apart, or NULL.
@@ -210,8 +210,9 @@ int32_t sf_moe_combine(int64_t tokens, int64_t cols, int32_t top_k, const void* 
 /* y[M,N] = act(x[M,K] . W[N,K]^T + bias) with
  *   W[n, k] = scales[k / group, n] * (q[n, k] - zeros[k / group, n]),
  * q in 0..15, zeros = 8 when NULL, for M <= 64 rows of bf16/fp16 x (the
- * weights are read once).  scales and zeros are [ceil(K / group)][lds >= N]
- * in x's type; group is 32, 64 or 128.  packed row n holds ldp >= 16 *
+ * weights are read once per 16 rows).  scales and zeros are
+ * [ceil(K / group)][lds >= N] in x's type; a zero stands for the whole number
+ * in 0..15 nearest to it; group is 32, 64 or 128.  packed row n holds ldp >= 16 *
  * ceil(K / 128) words (16-byte aligned, ldp a multiple of 4): nibble i (from
  * the low end) of word 4 t + w of 128-column block b holds column
  *   128 b + 32 w + 8 t + {0, 2, 4, 6, 1, 3, 5, 7}[i]

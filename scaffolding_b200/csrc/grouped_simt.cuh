@@ -7,47 +7,9 @@
 #pragma once
 #include <cstdint>
 
-#include "epilogue.cuh"
+#include "grouped_args.cuh"
 
 namespace sf {
-
-struct GroupedArgs {
-  int groups;
-  int M, N, K;            // N: columns of the output
-  const void* A;
-  int64_t a_rows, lda;
-  const int* rows;        // row of A of each output row, or null
-  const int* offsets;     // [groups + 1]
-  const void* B;          // [groups][N, or 2 N when gated][K]
-  int64_t ldb, b_stride;
-  const void* bias;       // [groups][N, or 2 N when gated], or null
-  int bias_dtype;
-  int64_t bias_stride;
-  void* C;
-  int64_t ldc;
-  int in_dtype, out_dtype;
-  int act;                // Act, or kActSiluGate
-  int fast_act;
-  int* err;
-};
-
-// Gated SiLU: y = silu(v[n]) * v[N + n]; the grouped GEMM's only, since it
-// pairs two weight rows for one output.
-constexpr int kActSiluGate = 3;
-
-// First and past-the-last row of group g.  Offsets are device data: each is
-// clamped to [0, M], so that no row outside the tensors is reached whatever
-// they hold.
-__device__ __forceinline__ void group_rows(const GroupedArgs& p, int g, int& lo, int& hi) {
-  lo = min(max(p.offsets[g], 0), p.M);
-  hi = max(lo, min(p.offsets[g + 1], p.M));
-}
-
-__device__ __forceinline__ float grouped_act(float v, float gate_up, int act, bool fast) {
-  if (act == kActSiluGate)
-    return (fast ? act_apply_fast(v, kActSilu) : act_apply(v, kActSilu)) * gate_up;
-  return fast ? act_apply_fast(v, act) : act_apply(v, act);
-}
 
 constexpr int kGsTile = 64, kGsK = 16, kGsThreads = 256;
 
@@ -55,17 +17,18 @@ template <bool GATE>
 static __global__ void __launch_bounds__(kGsThreads) grouped_simt_kernel(const GroupedArgs p) {
   __shared__ float As[kGsK][kGsTile + 4];
   __shared__ float Bs[GATE ? 2 : 1][kGsK][kGsTile + 4];
-  __shared__ int found[2];
+  __shared__ int found[3];
   const int n0 = blockIdx.x * kGsTile;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   // Tile blockIdx.y of the groups' tiles laid end to end; the host launches
   // as many as there can be (a partial tile per group on top of M / 64).
   if (tid < 32) {
-    int at = 0, g_hit = -1, first = 0;
-    for (int g0 = 0; g0 < p.groups && g_hit < 0; g0 += 32) {
-      const int g = g0 + tid;
-      int lo = 0, hi = 0;
-      if (g < p.groups) group_rows(p, g, lo, hi);
+    int at = 0, floor = 0;
+    if (tid == 0) found[0] = -1;
+    __syncwarp();
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+      int lo, hi;
+      group_bounds(p, g0, floor, lo, hi);
       const int tiles = (hi - lo + kGsTile - 1) / kGsTile;
       int end = tiles;
 #pragma unroll
@@ -76,23 +39,20 @@ static __global__ void __launch_bounds__(kGsThreads) grouped_simt_kernel(const G
       end += at;
       const unsigned past = __ballot_sync(0xffffffffu, end > static_cast<int>(blockIdx.y));
       if (past) {
-        const int l = __ffs(past) - 1;
-        g_hit = g0 + l;
-        first = __shfl_sync(0xffffffffu, end - tiles, l);
+        if (tid == __ffs(past) - 1) {
+          found[0] = g0 + tid;
+          found[1] = lo + (static_cast<int>(blockIdx.y) - (end - tiles)) * kGsTile;
+          found[2] = hi;
+        }
+        break;
       }
       at = __shfl_sync(0xffffffffu, end, 31);
-    }
-    if (tid == 0) {
-      found[0] = g_hit;
-      found[1] = static_cast<int>(blockIdx.y) - first;
     }
   }
   __syncthreads();
   const int g = found[0];
   if (g < 0) return;
-  int lo, hi;
-  group_rows(p, g, lo, hi);
-  const int m0 = lo + found[1] * kGsTile;
+  const int m0 = found[1], hi = found[2];
   const int64_t brow = static_cast<int64_t>(g) * p.b_stride;
 
   // The row of A that this thread stages (four threads per row).
