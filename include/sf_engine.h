@@ -172,13 +172,22 @@ int32_t sf_linear_skinny_noalloc(int64_t M, int64_t N, int64_t K,
  *   groups b_stride apart; bias likewise, bias_stride apart, or NULL.
  * 16-bit operands whose rows start on 16-byte boundaries run on the tensor
  * cores; fp32 and other layouts on the FMA pipe (IEEE fp32).  At most 4096
- * groups.  No counterpart in the reference, whose batched products
- * (_cuda_ops.pyx:1122-1190) have one size for the whole batch. */
+ * groups.  The workspace is optional: with
+ * sf_gemm_grouped_workspace_size() bytes of it (16-byte aligned), a call with
+ * many rows to gather copies them there first (one launch more), without it
+ * they are gathered as they are read; the result is the same, bit for bit.
+ * The size is 0 while `stream` is being captured, so that a graph never holds
+ * a workspace that something else uses.  No counterpart in the reference,
+ * whose batched products (_cuda_ops.pyx:1122-1190) have one size for the
+ * whole batch. */
 int32_t sf_gemm_grouped(int64_t groups, int64_t M, int64_t N, int64_t K, const void* A,
                         int64_t a_rows, int64_t lda, const int32_t* rows, const int32_t* offsets,
                         const void* B, int64_t ldb, int64_t b_stride, const void* bias,
                         int32_t bias_dtype, int64_t bias_stride, void* C, int64_t ldc,
-                        int32_t in_dtype, int32_t out_dtype, int32_t activation, void* stream);
+                        int32_t in_dtype, int32_t out_dtype, int32_t activation,
+                        void* workspace, size_t workspace_bytes, void* stream);
+int32_t sf_gemm_grouped_workspace_size(int64_t groups, int64_t M, int64_t N, int64_t K,
+                                       int32_t in_dtype, void* stream, size_t* bytes);
 
 /* Router: the top_k experts of every token by logit (falling; ties to the
  * lowest expert; NaN counts as -inf), their weights, and the choices grouped

@@ -534,10 +534,20 @@ def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTen
     y = _result(out, (M, N), odt, dev, "out")
     bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
     with E.on_device(dev):
+        ws, ws_bytes = None, 0
+        if rows is not None:
+            need = C.c_size_t()
+            check(lib.sf_gemm_grouped_workspace_size(X, M, N, K, E.dtype_code(gt_x.dtype),
+                                                     _stream_arg(dev), C.byref(need)),
+                  "sf_gemm_grouped_workspace_size")
+            if need.value:
+                buf = E.workspace(dev, E.get_stream(dev), need.value)
+                ws, ws_bytes = C.c_void_p(buf.ptr), buf.nbytes
         check(lib.sf_gemm_grouped(X, M, N, K, _ptr(gt_x), gt_x.shape[0], K, _ptr(rows),
                                   _ptr(gt_offsets), _ptr(gt_weight), K, wide * K, _ptr(gt_bias),
                                   bias_dt, wide, _ptr(y), N, E.dtype_code(gt_x.dtype),
-                                  E.dtype_code(odt), act, _stream_arg(dev)), "sf_gemm_grouped")
+                                  E.dtype_code(odt), act, ws, ws_bytes, _stream_arg(dev)),
+              "sf_gemm_grouped")
     return y
 
 

@@ -75,7 +75,8 @@ SIGNATURES: dict[str, list] = {
                                  _i32, _i32, _i32, _vp],
     "sf_gemm_workspace_size": [_P(Batch), _i64, _i64, _i64, _i32, _i32, _i32, _i32, _P(_sz)],
     "sf_gemm_grouped": [_i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
-                        _i32, _i64, _vp, _i64, _i32, _i32, _i32, _vp],
+                        _i32, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _sz, _vp],
+    "sf_gemm_grouped_workspace_size": [_i64, _i64, _i64, _i64, _i32, _vp, _P(_sz)],
     "sf_moe_route_workspace_size": [_i64, _i64, _i32, _P(_sz)],
     "sf_moe_route": [_i64, _i64, _i32, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                      _vp],

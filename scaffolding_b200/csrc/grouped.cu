@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.h"
 #include "grouped_simt.cuh"
@@ -19,6 +20,11 @@ namespace sf {
 namespace {
 
 constexpr int64_t kMaxGroups = 4096;
+// Mean rows per group up to which the narrow tiles are used (64 columns, or 32
+// of both halves).  Narrow / wide tiles, K = 2048, N = 1408, 64 experts: 66.5 /
+// 71.3 us at 16 rows per group, 77.8 / 74.9 us at 28; gated 104 / 114 us at 12.5
+// and 127 / 117 us at 28.
+constexpr int64_t kFewRows = 16;
 
 int32_t run_simt(const GroupedArgs& a, cudaStream_t s) {
   const int64_t row_tiles = ceil_div(a.M, kGsTile) + std::min(a.groups, a.M);
@@ -50,43 +56,128 @@ int32_t encode_rows(CUtensorMap* m, const GroupedArgs& a, uint32_t box_rows) {
   return SF_OK;
 }
 
+// Rows to gather from which they are copied into grouped order first, when
+// there is a workspace.  In the kernel every weight block gathers its rows
+// again through the load/store path, which costs 29 % over TMA boxes at 35552
+// rows (K = 1920, N = 7680: 1198 against 910 us) and is worth one pass over
+// the rows (45 us there) from about 2000 rows and 8 weight blocks on (3000
+// rows: 87 against 77 + 5 us; 800 rows: 27 against 25 + 3).
+constexpr int64_t kGatherFirstRows = 2048;
+constexpr int64_t kGatherFirstCols = 1024;
+
+bool gather_pays(int64_t groups, int64_t M, int64_t N) {
+  return M >= kGatherFirstRows && M > kFewRows * groups && N >= kGatherFirstCols;
+}
+
+// Elements of a gathered row: K rounded up to 16 bytes.
+int64_t gathered_ld(int64_t K) { return (K + 7) / 8 * 8; }
+
+// out[i, :] = A[rows[i], :], zeros for an index outside A; 16 bytes per thread
+// and step.  What lies past K in a row's last vector is copied along (it is
+// inside the row of A, which starts on 16-byte boundaries) and not used.
+__global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* A, int64_t ld_vec, int64_t a_rows,
+                                                          const int* rows, int M, int vecs, uint4* out) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t total = static_cast<int64_t>(M) * vecs;
+  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const int m = static_cast<int>(i / vecs), v = static_cast<int>(i - static_cast<int64_t>(m) * vecs);
+    const int64_t r = rows[m];
+    out[i] = r >= 0 && r < a_rows ? __ldg(A + r * ld_vec + v) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+int32_t gather_first(GroupedArgs& a, void* ws, const DeviceInfo& dev, cudaStream_t s) {
+  const int vecs = static_cast<int>(gathered_ld(a.K) / 8);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(
+      std::min<int64_t>(ceil_div(static_cast<int64_t>(a.M) * vecs, 256), dev.sm_count * 16LL)));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  SF_CUDA_TRY(cudaLaunchKernelEx(&cfg, gather_rows_kernel, static_cast<const uint4*>(a.A), a.lda / 8,
+                                 a.a_rows, a.rows, a.M, vecs, static_cast<uint4*>(ws)));
+  a.A = ws;
+  a.a_rows = a.M;
+  a.lda = gathered_ld(a.K);
+  a.rows = nullptr;
+  return SF_OK;
+}
+
+// Most tiles that M rows in `groups` groups can make, whatever the offsets say.
+int64_t most_tiles(const GroupedArgs& a, int bn) {
+  return (a.M / bn + std::min(a.groups, a.M)) * ceil_div(a.N, 128);
+}
+
 template <class Cfg>
-int32_t launch_tc(const GroupedArgs& a, const DeviceInfo& dev, int device, cudaStream_t s) {
-  const int64_t n_tiles = ceil_div(a.N, 128);
-  const int64_t most = (ceil_div(a.M, Cfg::BN) + std::min(a.groups, a.M)) * n_tiles;
-  if (most > INT32_MAX) return fail(SF_ERR_UNSUPPORTED, "%lld tiles exceed 2^31-1", (long long)most);
+int32_t launch_tc(GroupedArgs a, const DeviceInfo& dev, int device, cudaStream_t s) {
+  const int64_t most = most_tiles(a, Cfg::BN);
+  if (most > INT32_MAX / 8) return fail(SF_ERR_UNSUPPORTED, "%lld tiles exceed 2^28", (long long)most);
   const int64_t wide = Cfg::GATE ? 2LL * a.N : a.N;
   MapSpec w{a.B, 2, tma_dtype(a.in_dtype), static_cast<uint64_t>(a.K), static_cast<uint64_t>(wide),
             static_cast<uint64_t>(a.groups), 1, a.ldb, a.b_stride, 0, 64, 128};
   CUtensorMap mw, mx;
   int32_t st = encode_map(&mw, w);
-  if (st == SF_OK) st = encode_rows(&mx, a, a.rows ? 1 : Cfg::BOX);
+  if (st == SF_OK) st = encode_rows(&mx, a, Cfg::BOX);
   if (st != SF_OK) return st;
-  // The groups' first rows and tiles follow the ring.
-  const size_t smem = Cfg::RING_BYTES + 2 * (static_cast<size_t>(a.groups) + 1) * sizeof(int);
-  static size_t allowed[64] = {0};
   if (device >= 64) return fail(SF_ERR_UNSUPPORTED, "device index %d", device);
+  // The groups' first rows and tiles follow the ring.
   constexpr size_t kMost = Cfg::RING_BYTES + 2 * (kMaxGroups + 1) * sizeof(int);
   static_assert(kMost + 512 <= 227 * 1024, "shared memory budget");
-  if (allowed[device] == 0) {
+  static std::atomic<bool> allowed[64];
+  if (!allowed[device].load(std::memory_order_acquire)) {
     SF_CUDA_TRY(cudaFuncSetAttribute(grouped_tc_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      static_cast<int>(kMost)));
-    allowed[device] = kMost;
+    allowed[device].store(true, std::memory_order_release);
   }
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(most, dev.sm_count));
-  grouped_tc_kernel<Cfg><<<grid, Cfg::THREADS, smem, s>>>(mw, mx, a);
-  SF_CUDA_TRY(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(Cfg::SPLIT ? most * a.splits : std::min<int64_t>(most, dev.sm_count)));
+  cfg.blockDim = dim3(Cfg::THREADS + (a.rows ? 32 * Cfg::GATHER_WARPS : 0));
+  cfg.dynamicSmemBytes = Cfg::RING_BYTES + 2 * (static_cast<size_t>(a.groups) + 1) * sizeof(int);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(a.splits);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = Cfg::SPLIT ? 2 : 1;
+  SF_CUDA_TRY(cudaLaunchKernelEx(&cfg, grouped_tc_kernel<Cfg>, mw, mx, a));
   return SF_OK;
+}
+
+// CTAs per tile: where the tiles leave SMs idle, a tile's k-blocks (four at
+// least each) are shared by a cluster of 2, 4 or 8.  Clusters fill a GPC's SMs
+// only in part, and one that has to wait costs more than it saves: measured at
+// K = 7680, 16 tiles: 47 us alone, 28 / 17 / 22 us in clusters of 2 / 4 / 8;
+// 4 tiles of K = 4096: 26, 17 / 11 / 8.5 us; 22 tiles of K = 2048: 15, 11 / 8.9
+// / 14.5 us.
+int pick_splits(const GroupedArgs& a, int bn, int sm_count) {
+  const int64_t most = most_tiles(a, bn), kb = ceil_div(a.K, 64);
+  int s = 1;
+  while (s < 8 && most * s * 2 <= (s == 1 ? sm_count : s == 2 ? sm_count * 3 / 4 : sm_count / 3) &&
+         kb >= s * 8)
+    s *= 2;
+  return s;
+}
+
+template <int FMT, bool GATE, int BN_FEW, int STAGES_FEW, int BN, int STAGES>
+int32_t run_tc_sized(GroupedArgs a, const DeviceInfo& dev, int device, cudaStream_t s) {
+  if (a.M > kFewRows * a.groups) return launch_tc<GroupedCfg<BN, STAGES, FMT, GATE>>(a, dev, device, s);
+  a.splits = pick_splits(a, BN_FEW, dev.sm_count);
+  return a.splits > 1 ? launch_tc<GroupedCfg<BN_FEW, STAGES_FEW, FMT, GATE, true>>(a, dev, device, s)
+                      : launch_tc<GroupedCfg<BN_FEW, STAGES_FEW, FMT, GATE>>(a, dev, device, s);
 }
 
 template <int FMT>
 int32_t run_tc(const GroupedArgs& a, const DeviceInfo& dev, int device, cudaStream_t s) {
-  const bool few = a.M <= 32LL * a.groups;
-  if (a.act == kActSiluGate)
-    return few ? launch_tc<GroupedCfg<32, 5, FMT, true>>(a, dev, device, s)
-               : launch_tc<GroupedCfg<128, 4, FMT, true>>(a, dev, device, s);
-  return few ? launch_tc<GroupedCfg<32, 9, FMT, false>>(a, dev, device, s)
-             : launch_tc<GroupedCfg<256, 4, FMT, false>>(a, dev, device, s);
+  if (a.act == kActSiluGate) return run_tc_sized<FMT, true, 32, 5, 128, 4>(a, dev, device, s);
+  return run_tc_sized<FMT, false, 64, 8, 256, 4>(a, dev, device, s);
 }
 
 }  // namespace
@@ -99,7 +190,8 @@ extern "C" int32_t sf_gemm_grouped(int64_t groups, int64_t M, int64_t N, int64_t
                                    const int32_t* offsets, const void* B, int64_t ldb,
                                    int64_t b_stride, const void* bias, int32_t bias_dtype,
                                    int64_t bias_stride, void* C, int64_t ldc, int32_t in_dtype,
-                                   int32_t out_dtype, int32_t activation, void* stream) {
+                                   int32_t out_dtype, int32_t activation, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
   if (groups < 0 || M < 0 || N < 0 || K < 0 || a_rows < 0)
     return fail(SF_ERR_INVALID_ARGUMENT, "negative dimension");
   if (activation < SF_ACT_NONE || activation > SF_ACT_SILU_GATE)
@@ -151,5 +243,26 @@ extern "C" int32_t sf_gemm_grouped(int64_t groups, int64_t M, int64_t N, int64_t
                            bytes16(lda, 2) && bytes16(ldb, 2) && (groups == 1 || bytes16(b_stride, 2)) &&
                            b_stride >= 0;
   if (!describable) return run_simt(a, s);
+  const size_t gathered = static_cast<size_t>(M) * static_cast<size_t>(gathered_ld(K)) * 2;
+  if (rows && gather_pays(groups, M, N) && workspace && aligned16(workspace) && workspace_bytes >= gathered) {
+    const int32_t st2 = gather_first(a, workspace, *dev, s);
+    if (st2 != SF_OK) return st2;
+  }
   return in_dtype == kBF16 ? run_tc<1>(a, *dev, device, s) : run_tc<0>(a, *dev, device, s);
+}
+
+extern "C" int32_t sf_gemm_grouped_workspace_size(int64_t groups, int64_t M, int64_t N, int64_t K,
+                                                  int32_t in_dtype, void* stream, size_t* bytes) {
+  if (!bytes) return fail(SF_ERR_INVALID_ARGUMENT, "null output");
+  *bytes = 0;
+  if (groups < 0 || M < 0 || N < 0 || K < 0) return fail(SF_ERR_INVALID_ARGUMENT, "negative dimension");
+  if (in_dtype == kF32 || K == 0 || !gather_pays(groups, M, N)) return SF_OK;
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capturing) != cudaSuccess) {
+    cudaGetLastError();  // the legacy stream while another one is captured
+    return SF_OK;
+  }
+  if (capturing == cudaStreamCaptureStatusNone)
+    *bytes = static_cast<size_t>(M) * static_cast<size_t>(gathered_ld(K)) * 2;
+  return SF_OK;
 }

@@ -23,6 +23,7 @@ struct GroupedArgs {
   int in_dtype, out_dtype;
   int act;                // Act, or kActSiluGate
   int fast_act;
+  int splits;             // CTAs per tile of the split kernel
   int* err;
 };
 

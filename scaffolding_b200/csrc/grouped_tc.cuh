@@ -15,15 +15,19 @@
 // against the same rows into two accumulators, so both halves of an output
 // meet in one thread.
 //
-// Rows are gathered by TMA: one tile::gather4 copy fetches four rows of A by
-// index straight into the swizzled operand tile, and the gathered copy of A is
-// never written.  Without indices the rows come in boxes.  A copy that runs
-// past the group's end brings rows of the next group into columns that are
-// not stored.
+// Gathered rows are copied by index by one to eight more warps (10 on), 16
+// bytes per cp.async, into the swizzled operand tile; the copies arrive on the
+// stage's barrier themselves, and the MMA thread orders them before its reads.
+// (TMA's tile::gather4 does the same in one instruction per four rows, but
+// takes about 70 cycles for it: 4324 us where this takes 1198 us, 35552 rows of
+// 1920 against 8 experts of 7680.)  Without indices the rows come in TMA
+// boxes of 128 rows (16 in small tiles; boxes of 32 cost 16 % at that size).
+// A box that runs past the group's end brings rows of the next group into
+// columns that are not stored.
 //
-// CTA layout as the dense kernel (gemm_tc.cuh): warp 0 feeds the ring (all
-// lanes issue the row copies), warp 1 owns TMEM and issues the MMAs, warps 2-9
-// drain the accumulators, two of which let tile t + 1 start under t's stores.
+// CTA layout as the dense kernel (gemm_tc.cuh): warp 0 feeds the ring, warp 1
+// owns TMEM and issues the MMAs, warps 2-9 drain the accumulators, two of which
+// let tile t + 1 start under t's stores.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -35,23 +39,28 @@
 
 namespace sf {
 
-template <int BN_, int STAGES_, int FMT_, bool GATE_>
+template <int BN_, int STAGES_, int FMT_, bool GATE_, bool SPLIT_ = false>
 struct GroupedCfg {
   static constexpr int BM = 128;
   static constexpr int BN = BN_;  // most rows of a group in one tile
   static constexpr int STAGES = STAGES_;
   static constexpr int FMT = FMT_;  // 0 f16, 1 bf16
   static constexpr bool GATE = GATE_;
+  static constexpr bool SPLIT = SPLIT_;  // a cluster of CTAs shares a tile's k-blocks
   static constexpr int HALVES = GATE ? 2 : 1;
   static constexpr int BK = 64;
-  static constexpr int BOX = BN <= 32 ? 16 : 32;  // rows per ungathered copy
+  static constexpr int BOX = BN <= 32 ? 16 : BN <= 64 ? 32 : 128;  // rows per ungathered copy
   static constexpr int A_BYTES = BM * 128;        // one weight block
   static constexpr int STAGE_BYTES = HALVES * A_BYTES + BN * 128;
   static constexpr int ACC_COLS = HALVES * BN;
-  static constexpr int TMEM_COLS = 2 * ACC_COLS <= 64 ? 64 : 2 * ACC_COLS <= 128 ? 128 : 512;
-  static constexpr int CH = BN < 64 ? 16 : 32;  // accumulator columns per load
+  static constexpr int TMEM_COLS = 2 * ACC_COLS <= 64 ? 64 : 2 * ACC_COLS <= 128 ? 128 : 2 * ACC_COLS <= 256 ? 256 : 512;
+  static constexpr int CH = BN <= 32 ? 16 : 32;  // accumulator columns per load
   static constexpr int EPI_THREADS = 256;
-  static constexpr int THREADS = 64 + EPI_THREADS;
+  static constexpr int THREADS = 64 + EPI_THREADS;  // without the gather warps
+  // One 16-byte copy per row and lane keeps one warp busy up to 32 rows; more
+  // arrivals per stage than the rows need cost time (1 against 8 warps at 2 rows
+  // per group: 46.8 / 50.4 us).
+  static constexpr int GATHER_WARPS = BN <= 32 ? 1 : BN <= 64 ? 2 : 8;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES + 1024;  // + alignment slack
   static_assert(BN % 32 == 0 && BN <= 256 && 2 * ACC_COLS <= 512, "TMEM columns");
 };
@@ -88,16 +97,18 @@ struct GroupedTiles {
   }
 };
 
-// Four rows of a 2-D tensor by index, 128 bytes of each, into consecutive
-// 128-byte rows of a swizzled tile.  The map's box is one row high.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint64_t* bar,
-                                            int x, int r0, int r1, int r2, int r3) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(r0), "r"(r1), "r"(r2),
-      "r"(r3)
-      : "memory");
+// 16 bytes global -> shared, of which the first `bytes` are read and the rest
+// are zeros.
+__device__ __forceinline__ void gather_copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+
+// The float at shared::cta address `addr` of CTA `rank` of the cluster.
+__device__ __forceinline__ float load_cluster_f32(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(addr, rank)) : "memory");
+  return v;
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x,
@@ -110,9 +121,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
 }
 
 // tmW: weights {K, rows per group, groups}, box {64, 128}.  tmX: A {K, a_rows},
-// box {64, 1} for the gather, {64, BOX} otherwise.
+// box {64, BOX}; not used when the rows are gathered.  Launched with
+// Cfg::THREADS threads, and the gather warps on top when p.rows is given.
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::THREADS, 1)
+__global__ void __launch_bounds__(Cfg::THREADS + 32 * Cfg::GATHER_WARPS, 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                       const GroupedArgs p) {
   constexpr int BN = Cfg::BN, BK = Cfg::BK, STAGES = Cfg::STAGES, HALVES = Cfg::HALVES;
@@ -134,10 +146,11 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int n_tiles = (p.N + 127) / 128;
+  pdl_launch_dependents();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], p.rows ? 1 + 32 * Cfg::GATHER_WARPS : 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -154,6 +167,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     tmem_alloc(&tmem_slot, Cfg::TMEM_COLS);
     tmem_relinquish();
   }
+  pdl_wait();  // offsets, rows, A and C belong to the previous grid until it completes
   if (warp == 2) {
     // First row and tile of every group, 32 groups at a time.
     int at = 0, floor = 0;
@@ -185,73 +199,110 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   volatile int* abortp = &abort_flag;
   const GroupedTiles<BN> tiles{p.groups, firsts, starts};
   const int k_blocks = (p.K + BK - 1) / BK;
+  // Tiles u0, u0 + step, ... and the k-blocks of each that are this CTA's: all,
+  // or in a cluster of p.splits CTAs the rank's share of one tile (the host
+  // launches a cluster for every tile that there can be).
+  int u0 = blockIdx.x, step = gridDim.x, kb0 = 0, kb1 = k_blocks;
+  uint32_t rank = 0;
+  if constexpr (Cfg::SPLIT) {
+    rank = cluster_ctarank();
+    u0 = blockIdx.x / p.splits;
+    step = INT_MAX / 2;
+    const int per = (k_blocks + p.splits - 1) / p.splits;
+    kb0 = min(k_blocks, static_cast<int>(rank) * per);
+    kb1 = min(k_blocks, kb0 + per);
+  }
 
   if (warp == 0) {
-    // ───────────── producer ─────────────
-    int stage = 0;
-    uint32_t phase = 0;
-    int issued = 0;
-    bool ok = true;
-    GroupedTile t;
-    for (int u = blockIdx.x; ok && tiles.get(u, t); u += gridDim.x) {
-      // Lane l copies rows 8 l .. 8 l + 7 of the tile (two gathers), or box l.
-      const int gathers = (t.rows + 3) / 4, boxes = (t.rows + Cfg::BOX - 1) / Cfg::BOX;
-      int idx[8];
-      uint32_t bytes = HALVES * Cfg::A_BYTES;
-      if (p.rows) {
-        bytes += gathers * 512;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = 8 * lane + j;
-          int i = r < t.rows ? p.rows[t.row0 + r] : 0;
-          // an index outside A reads zeros, as does any past the last row
-          idx[j] = i < 0 || i >= p.a_rows ? static_cast<int>(p.a_rows) : i;
-        }
-      } else {
-        bytes += boxes * Cfg::BOX * 128;
-      }
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        if (lane == 0) ok = mbar_wait(&empty_bar[stage], phase ^ 1u, p.err, kDevTimeoutProducer, abortp);
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (!ok) break;
-        uint8_t* sw = smem + stage * Cfg::STAGE_BYTES;
-        const uint32_t sx = smem_u32(sw + HALVES * Cfg::A_BYTES);
-        if (lane == 0) {
+    // ───────────── TMA producer ─────────────
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      bool ok = true;
+      GroupedTile t;
+      for (int u = u0; ok && tiles.get(u, t); u += step) {
+        const int boxes = p.rows ? 0 : (t.rows + Cfg::BOX - 1) / Cfg::BOX;
+        const uint32_t bytes = HALVES * Cfg::A_BYTES + boxes * Cfg::BOX * 128;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.err, kDevTimeoutProducer, abortp)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sw = smem + stage * Cfg::STAGE_BYTES;
+          const uint32_t sx = smem_u32(sw + HALVES * Cfg::A_BYTES);
           mbar_arrive_expect_tx(&full_bar[stage], bytes);
           tma_load_4d(sw, &tmW, &full_bar[stage], kb * BK, t.n0, t.g, 0);
           if constexpr (Cfg::GATE)
             tma_load_4d(sw + Cfg::A_BYTES, &tmW, &full_bar[stage], kb * BK, p.N + t.n0, t.g, 0);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(sx + b * Cfg::BOX * 128, &tmX, &full_bar[stage], kb * BK, t.row0 + b * Cfg::BOX);
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
-        __syncwarp();
-        if (p.rows) {
+      }
+      if (!ok) {
+        // Abort: wait (bounded) for the copies still in flight.
+        const int n = issued < STAGES ? issued : STAGES;
+        int s = stage;
+        uint32_t ph = phase;
+        for (int j = 0; j < n; ++j) {
+          if (--s < 0) {
+            s = STAGES - 1;
+            ph ^= 1u;
+          }
+          if (!mbar_wait_quiet(&full_bar[s], ph, 200000000ull)) atomicCAS(p.err, 0, kDevTimeoutDrain);
+        }
+      }
+    }
+  } else if (warp >= 10) {
+    // ───────────── gather (warps 10..17) ─────────────
+    // Eight threads per row, 16 bytes each; thread i takes rows i / 8 + RP j.
+    constexpr int RP = 4 * Cfg::GATHER_WARPS, J = BN / RP;
+    const int i = threadIdx.x - Cfg::THREADS;
+    const int r0 = i >> 3, c = i & 7;
+    const uint32_t dst0 = r0 * 128 + ((c ^ (r0 & 7)) << 4);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    GroupedTile t;
+    for (int u = u0; ok && tiles.get(u, t); u += step) {
+      const uint16_t* from[J];
+      uint32_t live = 0;  // rows that exist
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (2 * lane + h < gathers)
-              tma_gather4(sx + (2 * lane + h) * 512, &tmX, &full_bar[stage], kb * BK, idx[4 * h],
-                          idx[4 * h + 1], idx[4 * h + 2], idx[4 * h + 3]);
-        } else if (lane < boxes) {
-          tma_load_2d(sx + lane * Cfg::BOX * 128, &tmX, &full_bar[stage], kb * BK, t.row0 + lane * Cfg::BOX);
+      for (int j = 0; j < J; ++j) {
+        const int r = r0 + RP * j;
+        const int row = r < t.rows ? p.rows[t.row0 + r] : -1;
+        const bool in = row >= 0 && row < p.a_rows;
+        live |= in ? 1u << j : 0u;
+        from[j] = static_cast<const uint16_t*>(p.A) + (in ? row * p.lda + kb0 * BK + 8 * c : 0);
+      }
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (lane == 0) ok = mbar_wait(&empty_bar[stage], phase ^ 1u, p.err, kDevTimeoutProducer, abortp);
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+        const uint32_t dst = smem_u32(smem + stage * Cfg::STAGE_BYTES + HALVES * Cfg::A_BYTES);
+        const int in_row = min(max(p.K - (kb * BK + 8 * c), 0), 8) * 2;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (RP * j >= t.rows) break;
+          const int bytes = (live >> j) & 1u ? in_row : 0;
+          // RP j rows further on; with RP = 4 every other one is in the swizzle's other half
+          gather_copy16(dst + j * (RP * 128) + (dst0 ^ (((RP * j) & 7) << 4)), from[j], bytes);
+          from[j] += BK;
         }
-        ++issued;
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[stage]))
+                     : "memory");
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
         }
       }
     }
-    if (!ok && lane == 0) {
-      // Abort: wait (bounded) for the copies still in flight.
-      const int n = issued < STAGES ? issued : STAGES;
-      int s = stage;
-      uint32_t ph = phase;
-      for (int j = 0; j < n; ++j) {
-        if (--s < 0) {
-          s = STAGES - 1;
-          ph ^= 1u;
-        }
-        if (!mbar_wait_quiet(&full_bar[s], ph, 200000000ull)) atomicCAS(p.err, 0, kDevTimeoutDrain);
-      }
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 1) {
     // ───────────── MMA issuer ─────────────
     if (lane == 0) {
@@ -262,7 +313,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       bool ok = true;
       bool issued_any = false;
       GroupedTile t;
-      for (int u = blockIdx.x; ok && tiles.get(u, t); u += gridDim.x) {
+      for (int u = u0; ok && tiles.get(u, t); u += step) {
         const uint32_t idesc = make_idesc(Cfg::FMT, 128, (t.rows + 15) / 16 * 16, 0u, 0u);
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, p.err, kDevTimeoutMma, abortp)) {
           ok = false;
@@ -270,11 +321,12 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * Cfg::ACC_COLS);
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, p.err, kDevTimeoutMma, abortp)) {
             ok = false;
             break;
           }
+          if (p.rows) fence_proxy_async_smem();  // the gathered rows were written by cp.async
           tc_fence_after();
           const uint32_t w_addr = smem_u32(smem + stage * Cfg::STAGE_BYTES);
           const uint32_t x_addr = w_addr + HALVES * Cfg::A_BYTES;
@@ -284,7 +336,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
               umma_f16(d + h * BN, make_sw128_desc(w_addr + h * Cfg::A_BYTES + ks * 32, 16, 1024), xd,
-                       idesc, (kb > 0 || ks > 0) ? 1u : 0u);
+                       idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
           }
           issued_any = true;
           umma_commit(&empty_bar[stage]);
@@ -313,7 +365,24 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     int acc = 0;
     uint32_t acc_phase = 0;
     GroupedTile t;
-    for (int u = blockIdx.x; tiles.get(u, t); u += gridDim.x) {
+    for (int u = u0; tiles.get(u, t); u += step) {
+      if constexpr (Cfg::SPLIT) {
+        // The partial sums take the ring's place: every copy into it was
+        // waited for and every MMA that read it has completed.
+        if (kb0 >= kb1) break;
+        if (!mbar_wait(&tfull_bar[0], 0, p.err, kDevTimeoutEpilogue, abortp)) break;
+        tc_fence_after();
+        float* part = reinterpret_cast<float*>(smem) + quad * 32 + lane;
+        for (int c = half * CH; c < t.rows; c += 2 * CH)
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h) {
+            float v[CH];
+            tmem_load_chunk<CH>(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + h * BN + c, v);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) part[(h * BN + c + i) * 128] = v[i];
+          }
+        break;
+      }
       const int n = t.n0 + quad * 32 + lane;  // this thread's weight row
       float bias0 = 0.0f, bias1 = 0.0f;
       if (p.bias && n < p.N) {
@@ -355,6 +424,33 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+  if constexpr (Cfg::SPLIT) {
+    // Every CTA of the cluster sums every splits-th row of the tile over the
+    // cluster's shared memory, in rank order.
+    cluster_sync();
+    GroupedTile t;
+    if (tiles.get(u0, t)) {
+      const int per = (k_blocks + p.splits - 1) / p.splits;
+      const int ranks = (k_blocks + per - 1) / per;  // ranks with k-blocks
+      const int i = threadIdx.x & 127, n = t.n0 + i;
+      const uint32_t part = smem_u32(smem) + i * 4;
+      if (n < p.N)
+        for (int r = rank + p.splits * (threadIdx.x >> 7); r < t.rows; r += p.splits * (blockDim.x >> 7)) {
+          if (static_cast<int>(threadIdx.x >> 7) >= static_cast<int>(blockDim.x >> 7)) break;
+          float v[2] = {0.0f, 0.0f};
+          for (int s = 0; s < ranks; ++s)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) v[h] += load_cluster_f32(part + (h * BN + r) * 512, s);
+          if (p.bias)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+              v[h] += load_as_f32(p.bias, t.g * p.bias_stride + h * p.N + n, p.bias_dtype);
+          store_from_f32(p.C, (static_cast<int64_t>(t.row0) + r) * p.ldc + n, p.out_dtype,
+                         grouped_act(v[0], v[1], p.act, p.fast_act != 0));
+        }
+    }
+    cluster_sync();  // no CTA leaves while its sums are being read
   }
 }
 

@@ -280,7 +280,7 @@ def test_grouped_strides_of_the_c_abi(gpu, ops, dt):
     code = E.dtype_code(np_dtype(dt))
     check(lib.sf_gemm_grouped(X, M, N, K, C.c_void_p(gx.ptr), M, lda, None, C.c_void_p(go.ptr),
                               C.c_void_p(gw.ptr), ldb, bs, C.c_void_p(gb.ptr), code, N + 9,
-                              C.c_void_p(out.ptr), ldc, code, code, 1, None), "sf_gemm_grouped")
+                              C.c_void_p(out.ptr), ldc, code, code, 1, None, 0, None), "sf_gemm_grouped")
     y = to_host32(ops, out).astype(np.float64)
     dense = np.stack([w[g, :N * ldb].reshape(N, ldb)[:, :K] for g in range(X)])
     ref, tol = plain_grouped(x[:, :K], dense, offsets, b[:, :N], "silu", None, dt)

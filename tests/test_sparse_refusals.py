@@ -128,7 +128,7 @@ def test_c_abi_refuses():
     odd = C.c_void_p(4100)
     sz = C.c_size_t()
     assert lib.sf_moe_route_workspace_size(100, 8, 2, C.byref(sz)) == 0 and sz.value == 0
-    assert lib.sf_moe_route_workspace_size(1000, 8, 2, C.byref(sz)) == 0 and sz.value == 8 * 8 * 4
+    assert lib.sf_moe_route_workspace_size(1000, 8, 2, C.byref(sz)) == 0 and sz.value == 16 * 8 * 4
     assert lib.sf_moe_route(1000, 8, 2, p, 0, 8, 1, p, p, p, p, p, None, 0, None) == SF_ERR_WORKSPACE
     assert lib.sf_moe_route(10, 8, 2, p, 0, 7, 1, p, p, p, p, p, None, 0, None) == BAD
     assert lib.sf_moe_route(10, 8, 2, p, 5, 8, 1, p, p, p, p, p, None, 0, None) == BAD
@@ -137,7 +137,7 @@ def test_c_abi_refuses():
 
     def grouped(groups=2, M=4, N=8, K=8, a_rows=4, lda=8, rows=None, off=p, ldb=8, ldc=8, dt=2, act=0, A=p):
         return lib.sf_gemm_grouped(groups, M, N, K, A, a_rows, lda, rows, off, p, ldb, 64, None, 0, 0, p,
-                                   ldc, dt, dt, act, None)
+                                   ldc, dt, dt, act, None, 0, None)
 
     assert grouped(M=-1) == BAD and grouped(act=4) == BAD and grouped(dt=3) == BAD
     assert grouped(off=None) == BAD and grouped(A=None) == BAD
