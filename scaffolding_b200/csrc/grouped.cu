@@ -72,18 +72,29 @@ bool gather_pays(int64_t groups, int64_t M, int64_t N) {
 // Elements of a gathered row: K rounded up to 16 bytes.
 int64_t gathered_ld(int64_t K) { return (K + 7) / 8 * 8; }
 
-// out[i, :] = A[rows[i], :], zeros for an index outside A; 16 bytes per thread
-// and step.  What lies past K in a row's last vector is copied along (it is
-// inside the row of A, which starts on 16-byte boundaries) and not used.
+// out[i, :] = A[rows[i], :], zeros for an index outside A; a warp per row, 16
+// bytes per lane and step.  What lies past K in a row's last vector is copied
+// along (it is inside the row of A, which starts on 16-byte boundaries) and
+// not used.
 __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* A, int64_t ld_vec, int64_t a_rows,
                                                           const int* rows, int M, int vecs, uint4* out) {
   pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
   pdl_wait();
-  const int64_t total = static_cast<int64_t>(M) * vecs;
-  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const int m = static_cast<int>(i / vecs), v = static_cast<int>(i - static_cast<int64_t>(m) * vecs);
+  for (int m = blockIdx.x * 8 + (threadIdx.x >> 5); m < M; m += gridDim.x * 8) {
     const int64_t r = rows[m];
-    out[i] = r >= 0 && r < a_rows ? __ldg(A + r * ld_vec + v) : make_uint4(0, 0, 0, 0);
+    const bool in = r >= 0 && r < a_rows;
+    const uint4* src = A + (in ? r * ld_vec : 0);
+    uint4* dst = out + static_cast<int64_t>(m) * vecs;
+    for (int v = lane; v < vecs; v += 128) {
+      uint4 u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        u[j] = in && v + 32 * j < vecs ? __ldg(src + v + 32 * j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v + 32 * j < vecs) dst[v + 32 * j] = u[j];
+    }
   }
 }
 
@@ -91,7 +102,7 @@ int32_t gather_first(GroupedArgs& a, void* ws, const DeviceInfo& dev, cudaStream
   const int vecs = static_cast<int>(gathered_ld(a.K) / 8);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(
-      std::min<int64_t>(ceil_div(static_cast<int64_t>(a.M) * vecs, 256), dev.sm_count * 16LL)));
+      std::min<int64_t>(ceil_div(a.M, 8), dev.sm_count * 8LL)));
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];

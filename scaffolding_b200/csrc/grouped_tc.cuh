@@ -120,6 +120,45 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// The activation of CH values, chosen once.
+template <int CH>
+__device__ __forceinline__ void activate(float (&v)[CH], int act, bool fast) {
+  if (act == kActNone) return;
+  if (!fast) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) v[i] = act_apply(v[i], act);
+  } else if (act == kActSilu) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) v[i] = act_apply_fast(v[i], kActSilu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) v[i] = act_apply_fast(v[i], kActGeluTanh);
+  }
+}
+
+// CH values of one output column: rows at, at + ld, ..., the first `left` of
+// them.  Neighbouring lanes hold neighbouring columns.
+template <int CH>
+__device__ __forceinline__ void store_column(void* C, int64_t at, int64_t ld, int dtype, const float (&v)[CH],
+                                             int left) {
+  if (dtype == kF32) {
+    float* p = static_cast<float*>(C) + at;
+#pragma unroll
+    for (int i = 0; i < CH; ++i, p += ld)
+      if (i < left) *p = v[i];
+  } else if (dtype == kBF16) {
+    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(C) + at;
+#pragma unroll
+    for (int i = 0; i < CH; ++i, p += ld)
+      if (i < left) *p = __float2bfloat16_rn(v[i]);
+  } else {
+    __half* p = static_cast<__half*>(C) + at;
+#pragma unroll
+    for (int i = 0; i < CH; ++i, p += ld)
+      if (i < left) *p = __float2half_rn(v[i]);
+  }
+}
+
 // tmW: weights {K, rows per group, groups}, box {64, 128}.  tmX: A {K, a_rows},
 // box {64, BOX}; not used when the rows are gathered.  Launched with
 // Cfg::THREADS threads, and the gather warps on top when p.rows is given.
@@ -395,19 +434,23 @@ __global__ void __launch_bounds__(Cfg::THREADS + 32 * Cfg::GATHER_WARPS, 1)
                              static_cast<uint32_t>(acc * Cfg::ACC_COLS);
 #pragma unroll 1
       for (int c = half * CH; c < t.rows; c += 2 * CH) {
-        float v[CH], w[Cfg::GATE ? CH : 1];
+        float v[CH];
         tmem_load_chunk<CH>(tbase + c, v);
-        if constexpr (Cfg::GATE) tmem_load_chunk<CH>(tbase + BN + c, w);
-        if (n < p.N) {
-          const int64_t at = static_cast<int64_t>(t.row0 + c) * p.ldc + n;
+        if constexpr (Cfg::GATE) {
+          float w[CH];
+          tmem_load_chunk<CH>(tbase + BN + c, w);
 #pragma unroll
           for (int i = 0; i < CH; ++i) {
-            if (c + i >= t.rows) break;
-            const float up = Cfg::GATE ? w[Cfg::GATE ? i : 0] + bias1 : 0.0f;
-            store_from_f32(p.C, at + i * p.ldc, p.out_dtype,
-                           grouped_act(v[i] + bias0, up, p.act, p.fast_act != 0));
+            const float z = v[i] + bias0;
+            v[i] = (p.fast_act ? act_apply_fast(z, kActSilu) : act_apply(z, kActSilu)) * (w[i] + bias1);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < CH; ++i) v[i] += bias0;
+          activate<CH>(v, p.act, p.fast_act != 0);
         }
+        if (n < p.N)
+          store_column<CH>(p.C, static_cast<int64_t>(t.row0 + c) * p.ldc + n, p.ldc, p.out_dtype, v, t.rows - c);
       }
       tc_fence_before();
       mbar_arrive(&tempty_bar[acc]);
