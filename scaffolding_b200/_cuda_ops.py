@@ -408,36 +408,36 @@ def dev_ada_layer_norm(gt: GpuTensor, gt_params: GpuTensor, gt_gamma: GpuTensor 
 
 # ───────────────────────────── experts ─────────────────────────────
 
-def _same_device(*tensors) -> int:
+_F32, _I32, _U32 = np.dtype(np.float32), np.dtype(np.int32), np.dtype(np.uint32)
+
+
+def _same_device(first: GpuTensor, *others) -> int:
     """Device of the tensors (None skipped); refuses a mix."""
-    devs = {t.device_id for t in tensors if t is not None}
-    if len(devs) != 1:
-        raise ValueError(f"operands on different devices ({' vs '.join(map(str, sorted(devs)))})")
-    return devs.pop()
+    dev = first.device_id
+    for t in others:
+        if t is not None and t.device_id != dev:
+            raise ValueError(f"operands on different devices ({dev} vs {t.device_id})")
+    return dev
 
 
 def _result(out, shape, dtype, dev, name: str) -> GpuTensor:
     """``out`` when the caller gives the result's buffer, else a new tensor."""
     if out is None:
         return _alloc(shape, dtype, dev)
-    if out.shape != tuple(shape) or out.dtype != np.dtype(dtype):
-        raise ValueError(f"{name} must be {tuple(shape)} {np.dtype(dtype)}, got {out.shape} {out.dtype}")
+    if out.shape != shape or out.dtype != dtype:
+        raise ValueError(f"{name} must be {shape} {dtype}, got {out.shape} {out.dtype}")
     return out
 
 
 def _int32(t: GpuTensor, name: str) -> GpuTensor:
-    if t.dtype != np.int32:
+    if t.dtype != _I32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
     return t
 
 
 def _ptr(t):
-    return C.c_void_p(t.ptr) if t is not None else None
-
-
-def _stream_arg(dev: int):
-    s = E.get_stream(dev)
-    return C.c_void_p(s) if s else None
+    """Address of a tensor, None for none (both as ctypes takes a pointer)."""
+    return t.buffer.ptr if t is not None else None
 
 
 class MoeRoute:
@@ -484,15 +484,15 @@ def dev_moe_route(gt_logits: GpuTensor, top_k: int, renormalize: bool = True,
         _same_device(gt_logits, out.experts, out.weights, out.offsets, out.rows, out.slots)
         for name, shape in (("experts", (T, k)), ("weights", (T, k)), ("offsets", (X + 1,)),
                             ("rows", (T * k,)), ("slots", (T, k))):
-            _result(getattr(out, name), shape, np.float32 if name == "weights" else np.int32, dev, name)
+            _result(getattr(out, name), shape, _F32 if name == "weights" else _I32, dev, name)
     if need.value and (out.scratch is None or out.scratch.nbytes < need.value
                        or out.scratch.device_id != dev):
         out.scratch = _make_buffer(need.value, dev)
-    ws = C.c_void_p(out.scratch.ptr) if need.value else None
+    ws = out.scratch.ptr if need.value else None
     with E.on_device(dev):
         check(lib.sf_moe_route(T, X, k, _ptr(gt_logits), code, X, 1 if renormalize else 0,
                                _ptr(out.experts), _ptr(out.weights), _ptr(out.offsets),
-                               _ptr(out.rows), _ptr(out.slots), ws, need.value, _stream_arg(dev)),
+                               _ptr(out.rows), _ptr(out.slots), ws, need.value, E.get_stream(dev)),
               "sf_moe_route")
     return out
 
@@ -538,15 +538,15 @@ def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTen
         if rows is not None:
             need = C.c_size_t()
             check(lib.sf_gemm_grouped_workspace_size(X, M, N, K, E.dtype_code(gt_x.dtype),
-                                                     _stream_arg(dev), C.byref(need)),
+                                                     E.get_stream(dev), C.byref(need)),
                   "sf_gemm_grouped_workspace_size")
             if need.value:
                 buf = E.workspace(dev, E.get_stream(dev), need.value)
-                ws, ws_bytes = C.c_void_p(buf.ptr), buf.nbytes
+                ws, ws_bytes = buf.ptr, buf.nbytes
         check(lib.sf_gemm_grouped(X, M, N, K, _ptr(gt_x), gt_x.shape[0], K, _ptr(rows),
                                   _ptr(gt_offsets), _ptr(gt_weight), K, wide * K, _ptr(gt_bias),
                                   bias_dt, wide, _ptr(y), N, E.dtype_code(gt_x.dtype),
-                                  E.dtype_code(odt), act, ws, ws_bytes, _stream_arg(dev)),
+                                  E.dtype_code(odt), act, ws, ws_bytes, E.get_stream(dev)),
               "sf_gemm_grouped")
     return y
 
@@ -561,7 +561,7 @@ def dev_moe_combine(gt_y: GpuTensor, gt_slots: GpuTensor, gt_weights: GpuTensor,
         raise ValueError(f"combine shapes: y {gt_y.shape}, slots {gt_slots.shape}")
     T, k = _int32(gt_slots, "slots").shape
     width = gt_y.shape[1]
-    if gt_weights.shape != (T, k) or gt_weights.dtype != np.float32:
+    if gt_weights.shape != (T, k) or gt_weights.dtype != _F32:
         raise ValueError(f"weights must be {(T, k)} float32, got {gt_weights.shape} {gt_weights.dtype}")
     if residual is not None and (residual.shape != (T, width) or residual.dtype != gt_y.dtype):
         raise ValueError(f"residual must be {(T, width)} {gt_y.dtype}, got {residual.shape} {residual.dtype}")
@@ -570,7 +570,7 @@ def dev_moe_combine(gt_y: GpuTensor, gt_slots: GpuTensor, gt_weights: GpuTensor,
     with E.on_device(dev):
         check(lib.sf_moe_combine(T, width, k, _ptr(gt_y), gt_y.shape[0], width,
                                  E.dtype_code(gt_y.dtype), _ptr(gt_slots), _ptr(gt_weights),
-                                 _ptr(residual), width, _ptr(o), width, _stream_arg(dev)),
+                                 _ptr(residual), width, _ptr(o), width, E.get_stream(dev)),
               "sf_moe_combine")
     return o
 
@@ -613,7 +613,7 @@ class W4Weight:
                  in_features: int, group: int = 128):
         if group not in (32, 64, 128):
             raise ValueError(f"group of {group} columns (32, 64 or 128)")
-        if packed.ndim != 2 or packed.dtype not in (np.dtype(np.uint32), np.dtype(np.int32)):
+        if packed.ndim != 2 or packed.dtype not in (_U32, _I32):
             raise ValueError(f"packed must be 2-d uint32, got {packed.shape} {packed.dtype}")
         n = packed.shape[0]
         if packed.shape[1] != -(-in_features // 128) * 16:
@@ -674,7 +674,7 @@ def dev_quantize_w4(gt_weight: GpuTensor, group: int = 128, zeros: bool = False,
     with E.on_device(dev):
         check(lib.sf_quantize_w4(n, k, _ptr(gt_weight), E.dtype_code(gt_weight.dtype), k, group,
                                  _ptr(packed), words, _ptr(scales), _ptr(zs), n,
-                                 E.dtype_code(sdt), _stream_arg(dev)), "sf_quantize_w4")
+                                 E.dtype_code(sdt), E.get_stream(dev)), "sf_quantize_w4")
     return W4Weight(packed, scales, zs, in_features=k, group=group)
 
 
@@ -689,7 +689,7 @@ def dev_dequantize_w4(weight: W4Weight, dtype=None) -> GpuTensor:
         check(lib.sf_dequantize_w4(n, k, _ptr(weight.packed), weight.packed.shape[1],
                                    _ptr(weight.scales), _ptr(weight.zeros), n, weight.group,
                                    E.dtype_code(weight.scales.dtype), _ptr(w), E.dtype_code(wdt), k,
-                                   _stream_arg(dev)), "sf_dequantize_w4")
+                                   E.get_stream(dev)), "sf_dequantize_w4")
     return w
 
 
@@ -703,7 +703,7 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
     act = E.act_code(activation)
     if gt_x.dtype != weight.scales.dtype:
         raise TypeError(f"x and the weight's scales must share a dtype ({gt_x.dtype} vs {weight.scales.dtype})")
-    if gt_x.dtype == np.float32:
+    if gt_x.dtype == _F32:
         raise TypeError("4-bit linears take bf16 or fp16 x")
     n, k = weight.shape
     if gt_x.ndim < 1 or gt_x.shape[-1] != k:
@@ -721,7 +721,7 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
             check(lib.sf_linear_w4(M, n, k, _ptr(gt_x), k, _ptr(weight.packed),
                                    weight.packed.shape[1], _ptr(weight.scales), _ptr(weight.zeros),
                                    n, weight.group, _ptr(gt_bias), bias_dt, _ptr(y), n, in_code,
-                                   out_code, act, _stream_arg(dev)), "sf_linear_w4")
+                                   out_code, act, E.get_stream(dev)), "sf_linear_w4")
         else:
             w = dev_dequantize_w4(weight)
             epi = E.make_epilogue(bias_ptr=gt_bias.ptr if gt_bias is not None else 0,

@@ -27,15 +27,18 @@ _ACTS = {"none": ACT_NONE, None: ACT_NONE, "silu": ACT_SILU, "gelu_tanh": ACT_GE
 _GROUPED_ACTS = {**_ACTS, "silu_gate": ACT_SILU_GATE}
 
 
+_DTYPE_CODES = {np.dtype(np.float32): DT_F32, np.dtype(np.float16): DT_F16}
+if bfloat16 is not None:
+    _DTYPE_CODES[bfloat16] = DT_BF16
+
+
 def dtype_code(dtype) -> int:
-    dt = np.dtype(dtype)
-    if dt == np.float32:
-        return DT_F32
-    if dt == np.float16:
-        return DT_F16
-    if bfloat16 is not None and dt == bfloat16:
-        return DT_BF16
-    raise TypeError(f"unsupported dtype for the matmul engine: {dt}")
+    code = _DTYPE_CODES.get(dtype)
+    if code is None:
+        code = _DTYPE_CODES.get(np.dtype(dtype))
+    if code is None:
+        raise TypeError(f"unsupported dtype for the matmul engine: {np.dtype(dtype)}")
+    return code
 
 
 def code_dtype(code: int) -> np.dtype:
