@@ -185,7 +185,6 @@ __global__ void __launch_bounds__(Cfg::THREADS + 32 * Cfg::GATHER_WARPS, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int n_tiles = (p.N + 127) / 128;
-  pdl_launch_dependents();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -234,6 +233,9 @@ __global__ void __launch_bounds__(Cfg::THREADS + 32 * Cfg::GATHER_WARPS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Only now: a dependent CTA that took TMEM first and waited for this grid
+  // would keep this one from getting its own.
+  pdl_launch_dependents();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abortp = &abort_flag;
   const GroupedTiles<BN> tiles{p.groups, firsts, starts};

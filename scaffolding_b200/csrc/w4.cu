@@ -16,41 +16,15 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
+#include <cstdlib>
 
 #include "common.h"
-#include "epilogue.cuh"
-#include "ptx.cuh"
 #include "tma_host.h"
+#include "w4_tc.cuh"
 
 namespace sf {
 namespace {
-
-constexpr int kW4MaxRows = 64;
-
-struct W4Args {
-  int M, N, K;
-  const void* x;
-  int64_t ldx;
-  const uint32_t* packed;
-  int64_t ldp;  // words per row
-  const void* scales;
-  const void* zeros;
-  int64_t lds;
-  int group;    // 32, 64 or 128
-  int dtype;    // of x, scales and zeros
-  const void* bias;
-  int bias_dtype;
-  void* y;
-  int64_t ldy;
-  int out_dtype;
-  int act;
-  int fast_act;
-};
-
-// Column, within its 128-column block, of nibble i of word j.
-__host__ __device__ __forceinline__ int w4_column(int j, int i) {
-  return 32 * (j & 3) + 8 * (j >> 2) + (i < 4 ? 2 * i : 2 * i - 7);
-}
 
 // ───────────────────────── up to 64 rows of x ─────────────────────────
 // Weights as the 16-row side of mma.m16n8k16, rows of x as its 8 columns: the
@@ -91,67 +65,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         "{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// (v & mask) | magic as the one logic operation that it is.
-__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(magic));
-  return r;
-}
-
-// A stored zero point as the whole number 0..15 it stands for.
-__device__ __forceinline__ float whole_zero(float z) { return fminf(fmaxf(rintf(z), 0.0f), 15.0f); }
-
-// Word -> four pairs (columns 2 i, 2 i + 1) of q - z.  z is the pair constant
-// of the group: 128 + z (bf16); 1024 + z in .x and 64 + z in .y (fp16).
-template <bool BF16>
-__device__ __forceinline__ void unpack_word(uint32_t w, uint2 z, uint32_t (&p)[4]) {
-  if constexpr (BF16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t v = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
-      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
-                                       *reinterpret_cast<const __nv_bfloat162*>(&z.x));
-      p[i] = *reinterpret_cast<const uint32_t*>(&d);
-    }
-  } else {
-    const uint32_t sixteenth = 0x2C002C00u;  // 1/16, 1/16
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t u = h ? w >> 8 : w;
-      const uint32_t lo = and_or(u, 0x000F000Fu, 0x64006400u);  // 1024 + q
-      const uint32_t hi = and_or(u, 0x00F000F0u, 0x64006400u);  // 1024 + 16 q
-      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&z.x));
-      const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi),
-                                *reinterpret_cast<const __half2*>(&sixteenth),
-                                __hneg2(*reinterpret_cast<const __half2*>(&z.y)));
-      p[2 * h] = *reinterpret_cast<const uint32_t*>(&a);
-      p[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-  }
-}
-
-// The pair constant of a stored zero point (16 bits, low half of v): adding
-// the magic rounds it to a whole number, the clamp keeps it in 0..15 (a NaN
-// becomes 0), as whole_zero does.
-template <bool BF16>
-__device__ __forceinline__ uint2 zero_pair(uint16_t v) {
-  const uint32_t two = static_cast<uint32_t>(v) * 0x10001u;
-  uint2 r;
-  if constexpr (BF16) {
-    __nv_bfloat162 m = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&two), __float2bfloat162_rn(128.0f));
-    m = __hmin2(__hmax2(m, __float2bfloat162_rn(128.0f)), __float2bfloat162_rn(143.0f));
-    r.x = *reinterpret_cast<const uint32_t*>(&m);
-    r.y = 0;
-  } else {
-    __half2 m = __hadd2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(1024.0f));
-    m = __hmin2(__hmax2(m, __float2half2_rn(1024.0f)), __float2half2_rn(1039.0f));
-    const __half2 n = __hsub2(m, __float2half2_rn(960.0f));
-    r.x = *reinterpret_cast<const uint32_t*>(&m);
-    r.y = *reinterpret_cast<const uint32_t*>(&n);
-  }
-  return r;
 }
 
 // Eight columns of x at p, of which `left` lie before K; 0 past them.
@@ -371,8 +284,93 @@ int32_t launch_w4_group(const W4Args& a, bool x_vec, cudaStream_t s) {
   return launch_w4<BF16, NT, 4>(a, x_vec, s);
 }
 
+// ───────────────────────── tcgen05 kernel ─────────────────────────
+
+int32_t encode_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, int64_t cols, int64_t rows,
+                  int64_t row_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t step[2] = {1, 1};
+  const CUresult r = fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): {%lld, %lld} rows of %lld bytes",
+                static_cast<int>(r), (long long)cols, (long long)rows, (long long)row_bytes);
+  return SF_OK;
+}
+
+// CTAs per row tile, which share its blocks.  A block takes a CTA about as long
+// next to another CTA as alone (it waits on its own MMAs), so what counts is the
+// number of waves of two CTAs per SM times the blocks of a CTA, plus about four
+// blocks' time for its start and end.  Measured, 64 rows of x: 4096 x 4096 34 /
+// 23 / 14 / 11 us in clusters of 1 / 2 / 4 / 8; 4096 -> 11008 49 / 29 / 22 / 31 us
+// in 1 / 2 / 3 / 4; 8192 -> 28672 75 / 80 / 85 / 101 us in 1 / 2 / 4 / 8.
+int pick_w4_splits(const W4Args& a, int sm_count) {
+  const int64_t tiles = ceil_div(a.N, 128), blocks = ceil_div(a.K, 128);
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= 8 && s <= blocks; ++s) {
+    const int64_t cost = ceil_div(tiles * s, 2 * sm_count) * (ceil_div(blocks, s) + 4);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+template <class Cfg>
+int32_t launch_w4_tc(const W4Args& a, const DeviceInfo& dev, int device, cudaStream_t s) {
+  const int n_rows = (a.M + 15) / 16 * 16;
+  const int64_t blocks = ceil_div(a.K, 128);
+  CUtensorMap mw, mx;
+  int32_t st = encode_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.packed, blocks * 16, a.N, a.ldp * 4, 16, 128,
+                         CU_TENSOR_MAP_SWIZZLE_64B);
+  if (st == SF_OK)
+    st = encode_2d(&mx, tma_dtype(a.dtype), a.x, a.K, a.M, a.ldx * 2, 64, n_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != SF_OK) return st;
+  if (device >= 64) return fail(SF_ERR_UNSUPPORTED, "device index %d", device);
+  static std::atomic<bool> allowed[64];
+  if (!allowed[device].load(std::memory_order_acquire)) {
+    SF_CUDA_TRY(cudaFuncSetAttribute(w4_tc_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     Cfg::SMEM_BYTES));
+    allowed[device].store(true, std::memory_order_release);
+  }
+  const int splits = pick_w4_splits(a, dev.sm_count);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(a.N, 128) * splits));
+  cfg.blockDim = dim3(Cfg::THREADS);
+  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  SF_CUDA_TRY(cudaLaunchKernelEx(&cfg, w4_tc_kernel<Cfg>, mw, mx, a, splits, n_rows, dev.err_word));
+  return SF_OK;
+}
+
+// Up to 16 rows of x run on mma.sync, more on tcgen05 (16 rows: 7.5 against 8.9
+// us at 4096 x 4096, 76 against 68 us at 8192 -> 28672; 33 rows: 213 against 69
+// us there).  Rows of x that TMA cannot describe take the former, 16 at a time.
 template <bool BF16>
 int32_t run_w4(const W4Args& a, cudaStream_t s) {
+  if (a.M > 16 && a.ldx % 8 == 0 && aligned16(a.x)) {
+    DeviceInfo* dev = nullptr;
+    int device = 0;
+    const int32_t st = current_device_info(&dev, &device);
+    if (st != SF_OK) return st;
+    if (a.group == 32) return launch_w4_tc<W4TcCfg<BF16, 1>>(a, *dev, device, s);
+    if (a.group == 64) return launch_w4_tc<W4TcCfg<BF16, 2>>(a, *dev, device, s);
+    return launch_w4_tc<W4TcCfg<BF16, 4>>(a, *dev, device, s);
+  }
   const bool x_vec = a.K % 8 == 0 && a.ldx % 8 == 0 && aligned16(a.x);
   if (a.M <= 8) return launch_w4_group<BF16, 1>(a, x_vec, s);
   W4Args p = a;

@@ -1,0 +1,97 @@
+// Arguments and unpacking of 4-bit weights, shared by the 4-bit linear kernels.
+#pragma once
+#include <cstdint>
+
+#include "epilogue.cuh"
+
+namespace sf {
+
+constexpr int kW4MaxRows = 64;
+
+struct W4Args {
+  int M, N, K;
+  const void* x;
+  int64_t ldx;
+  const uint32_t* packed;
+  int64_t ldp;  // words per row
+  const void* scales;
+  const void* zeros;
+  int64_t lds;
+  int group;    // 32, 64 or 128
+  int dtype;    // of x, scales and zeros
+  const void* bias;
+  int bias_dtype;
+  void* y;
+  int64_t ldy;
+  int out_dtype;
+  int act;
+  int fast_act;
+};
+
+// Column, within its 128-column block, of nibble i of word j.
+__host__ __device__ __forceinline__ int w4_column(int j, int i) {
+  return 32 * (j & 3) + 8 * (j >> 2) + (i < 4 ? 2 * i : 2 * i - 7);
+}
+
+// (v & mask) | magic as the one logic operation that it is.
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(magic));
+  return r;
+}
+
+// A stored zero point as the whole number 0..15 it stands for.
+__device__ __forceinline__ float whole_zero(float z) { return fminf(fmaxf(rintf(z), 0.0f), 15.0f); }
+
+// Word -> four pairs (columns 2 i, 2 i + 1) of q - z.  z is the pair constant
+// of the group: 128 + z (bf16); 1024 + z in .x and 64 + z in .y (fp16).
+template <bool BF16>
+__device__ __forceinline__ void unpack_word(uint32_t w, uint2 z, uint32_t (&p)[4]) {
+  if constexpr (BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&z.x));
+      p[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+  } else {
+    const uint32_t sixteenth = 0x2C002C00u;  // 1/16, 1/16
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t u = h ? w >> 8 : w;
+      const uint32_t lo = and_or(u, 0x000F000Fu, 0x64006400u);  // 1024 + q
+      const uint32_t hi = and_or(u, 0x00F000F0u, 0x64006400u);  // 1024 + 16 q
+      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&z.x));
+      const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi),
+                                *reinterpret_cast<const __half2*>(&sixteenth),
+                                __hneg2(*reinterpret_cast<const __half2*>(&z.y)));
+      p[2 * h] = *reinterpret_cast<const uint32_t*>(&a);
+      p[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+}
+
+// The pair constant of a stored zero point (16 bits, low half of v): adding
+// the magic rounds it to a whole number, the clamp keeps it in 0..15 (a NaN
+// becomes 0), as whole_zero does.
+template <bool BF16>
+__device__ __forceinline__ uint2 zero_pair(uint16_t v) {
+  const uint32_t two = static_cast<uint32_t>(v) * 0x10001u;
+  uint2 r;
+  if constexpr (BF16) {
+    __nv_bfloat162 m = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&two), __float2bfloat162_rn(128.0f));
+    m = __hmin2(__hmax2(m, __float2bfloat162_rn(128.0f)), __float2bfloat162_rn(143.0f));
+    r.x = *reinterpret_cast<const uint32_t*>(&m);
+    r.y = 0;
+  } else {
+    __half2 m = __hadd2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(1024.0f));
+    m = __hmin2(__hmax2(m, __float2half2_rn(1024.0f)), __float2half2_rn(1039.0f));
+    const __half2 n = __hsub2(m, __float2half2_rn(960.0f));
+    r.x = *reinterpret_cast<const uint32_t*>(&m);
+    r.y = *reinterpret_cast<const uint32_t*>(&n);
+  }
+  return r;
+}
+
+}  // namespace sf
