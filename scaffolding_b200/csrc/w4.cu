@@ -17,55 +17,28 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
+#include <climits>
+#include <utility>
 
 #include "common.h"
 #include "tma_host.h"
+#include "w4_stream.cuh"
 #include "w4_tc.cuh"
 
 namespace sf {
 namespace {
 
-// ───────────────────────── up to 64 rows of x ─────────────────────────
-// Weights as the 16-row side of mma.m16n8k16, rows of x as its 8 columns: the
-// product is bound by the weight stream (half a byte per weight against 16
-// multiply-adds at most 8 rows), and what has to keep up with it is the
-// unpacking.  At 6.5 TB/s a lane has 2.8 issue slots per weight.  A packed
-// word becomes four operand registers by masking two nibbles at a time into
-// the mantissas of 128 (bf16) or 1024 (fp16) and subtracting that plus the
-// zero point, which is exact: 1.1 to 1.4 operations per weight, one scale and
-// four multiply-adds per group, and the tensor core does the products.
-//
-// A warp owns 32 weight rows and every WK-th 128-column block of them.  In a
-// block, lane (g, t) = (lane / 4, lane % 4) takes 16 bytes of each of rows g,
-// g + 8, g + 16, g + 24: words 4 t .. 4 t + 3, whose columns 32 w + 8 t .. + 7
-// are one 16-byte piece of x for token g.  The order of k within an mma is free
-// as long as both operands agree, so the layout makes every copy of both
-// operands 16 bytes and word w of all four t one 32-column group.  Words and x
-// travel through a ring of asynchronous copies; scales are loaded two blocks
-// ahead, one row per lane.  The WK partial sums of a row meet in shared memory,
-// in warp order.  More than 16 rows of x run in passes of 16.
+// ───────────────────────── ring kernel ─────────────────────────
+// Up to 16 rows of x, any layout: the unpacking and the fragments of
+// w4_stream.cuh with less around them.  A warp owns 32 weight rows and every
+// WK-th block of them, and copies its lanes' words and x itself (16 bytes per
+// cp.async, kW4Stages blocks ahead); scales are loaded two blocks ahead, one row
+// per lane.  The WK partial sums of a row meet in shared memory, in warp order.
+// More than 16 rows of x run in passes of 16.
 
 constexpr int kW4Threads = 256;
 constexpr int kW4Rows = 32;   // weight rows of a warp
 constexpr int kW4Stages = 3;  // blocks in flight per warp
-
-template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                          uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 // Eight columns of x at p, of which `left` lie before K; 0 past them.
 __device__ __forceinline__ uint4 load_x8_ragged(const uint16_t* p, int left) {
@@ -95,6 +68,7 @@ __device__ __forceinline__ void copy_async_wait() {
 template <bool BF16, int NT, int GW>
 __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int wk, int x_vec) {
   constexpr int NG = 4 / GW;             // groups per block
+  constexpr int NA = w4_accumulators(NT, GW);
   constexpr int kSlot = (4 + 4 * NT) * 32;  // 16-byte vectors per block: a lane's words and x
   // Each lane's own words and x, kW4Stages blocks ahead: a lane reads back only
   // what it copied itself, so its own wait on the copies is all the order needed.
@@ -118,9 +92,8 @@ __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int 
   const uint16_t* xp = static_cast<const uint16_t*>(a.x) + g * a.ldx + 128 * kw + 8 * t;
   int left = a.K - (128 * kw + 8 * t);  // columns from xp to the row's end
   // scales and zeros of row n0 + lane, shared out by shuffles
-  const uint16_t* sp = static_cast<const uint16_t*>(a.scales) + kw * NG * a.lds + min(n0 + lane, a.N - 1);
-  const uint16_t* zp = static_cast<const uint16_t*>(a.zeros) + kw * NG * a.lds + min(n0 + lane, a.N - 1);
-  const int64_t s_step = static_cast<int64_t>(wk) * NG * a.lds;
+  const uint16_t* sp = static_cast<const uint16_t*>(a.scales) + min(n0 + lane, a.N - 1);
+  const uint16_t* zp = static_cast<const uint16_t*>(a.zeros) + min(n0 + lane, a.N - 1);
   const bool zeros = a.zeros != nullptr;
 
   int copied = 0;
@@ -151,20 +124,15 @@ __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int 
     copy_async_commit();
   };
   int scaled = 0;
-  uint16_t sc[3][NG], ze[3][NG];  // two blocks ahead
+  uint32_t sc[3][NG], ze[3][NG];  // two blocks ahead
   auto load_scales = [&](int to) {
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      const bool in = scaled < mine && (kw + scaled * wk) * NG + j < groups;
-      sc[to][j] = in ? __ldg(sp + j * a.lds) : 0;
-      ze[to][j] = in && zeros ? __ldg(zp + j * a.lds) : 0;
+      const int64_t at = min((kw + scaled * wk) * NG + j, groups - 1) * a.lds;  // past the last group: not used
+      sc[to][j] = load_ahead(sp + at);
+      if (zeros) ze[to][j] = load_ahead(zp + at);
     }
     ++scaled;
-    sp += s_step;
-    zp += s_step;
-  };
-  auto as_float = [](uint16_t v) {
-    return BF16 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v));
   };
   load_scales(0);
   load_scales(1);
@@ -179,7 +147,7 @@ __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int 
       uint2 zv[NG];
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        sv[j] = as_float(sc[u][j]);
+        sv[j] = (kw + (i0 + u) * wk) * NG + j < groups ? w4_float<BF16>(sc[u][j]) : 0.0f;
         if (zeros) zv[j] = zero_pair<BF16>(ze[u][j]);
       }
       load_scales((u + 2) % 3);
@@ -200,7 +168,7 @@ __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int 
             if constexpr (!BF16) z[r].y = __shfl_sync(0xffffffffu, zv[j].y, 8 * r + g);
           }
         }
-        float sum[2][NT][4] = {};
+        float sum[2][NT][NA][4] = {};
 #pragma unroll
         for (int l = 0; l < GW; ++l) {
           const int w = j * GW + l;
@@ -215,8 +183,8 @@ __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int 
             for (int r = 0; r < 2; ++r) {
               const uint32_t a0[4] = {p[2 * r][0], p[2 * r + 1][0], p[2 * r][1], p[2 * r + 1][1]};
               const uint32_t a1[4] = {p[2 * r][2], p[2 * r + 1][2], p[2 * r][3], p[2 * r + 1][3]};
-              mma_16816<BF16>(sum[r][n], a0, x.x, x.y);
-              mma_16816<BF16>(sum[r][n], a1, x.z, x.w);
+              mma_16816<BF16>(sum[r][n][2 * l % NA], a0, x.x, x.y);
+              mma_16816<BF16>(sum[r][n][2 * l % NA + 1], a1, x.z, x.w);
             }
           }
         }
@@ -226,7 +194,7 @@ __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int 
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              acc[r][n][c] = fmaf(s[2 * r + (c >> 1)], sum[r][n][c], acc[r][n][c]);
+              acc[r][n][c] = fmaf(s[2 * r + (c >> 1)], sum_of<NA>(sum[r][n], c), acc[r][n][c]);
       }
     }
   }
@@ -286,20 +254,110 @@ int32_t launch_w4_group(const W4Args& a, bool x_vec, cudaStream_t s) {
 
 // ───────────────────────── tcgen05 kernel ─────────────────────────
 
-int32_t encode_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, int64_t cols, int64_t rows,
-                  int64_t row_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+int32_t encode(CUtensorMap* m, CUtensorMapDataType dt, const void* base, int rank, const cuuint64_t* dims,
+               const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
-  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t step[2] = {1, 1};
-  const CUresult r = fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r = fn(m, dt, rank, const_cast<void*>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
-    return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): {%lld, %lld} rows of %lld bytes",
-                static_cast<int>(r), (long long)cols, (long long)rows, (long long)row_bytes);
+    return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): {%llu, %llu} rows of %llu bytes",
+                static_cast<int>(r), (unsigned long long)dims[0], (unsigned long long)dims[1],
+                (unsigned long long)strides[0]);
   return SF_OK;
+}
+
+// Packed words {16 per block, N}, boxes of one block of 128 rows.
+int32_t encode_words(CUtensorMap* m, const W4Args& a, CUtensorMapSwizzle swizzle) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(ceil_div(a.K, 128) * 16), static_cast<cuuint64_t>(a.N)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.ldp) * 4};
+  const cuuint32_t box[2] = {16, 128};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.packed, 2, dims, strides, box, swizzle);
+}
+
+// A launch in clusters of `splits` CTAs with programmatic stream serialisation.
+template <class Kernel, class... Args>
+int32_t launch_cluster(Kernel kernel, int64_t grid, int threads, size_t smem, int splits, cudaStream_t s,
+                       Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  SF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+  return SF_OK;
+}
+
+// The opt-in to a kernel's dynamic shared memory, once per device.
+template <class Kernel>
+int32_t allow_smem(Kernel kernel, int bytes, int device, std::atomic<bool> (&allowed)[64]) {
+  if (device >= 64) return fail(SF_ERR_UNSUPPORTED, "device index %d", device);
+  if (!allowed[device].load(std::memory_order_acquire)) {
+    SF_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    allowed[device].store(true, std::memory_order_release);
+  }
+  return SF_OK;
+}
+
+// Blocks of 128 x 128 from which the streaming kernel is used.  Its clusters and
+// its CTA-wide pipeline cost about 3 us more to start and to end than the ring
+// kernel's, and it streams faster.  Ring / stream, one row of x, group 128: 5.1 /
+// 6.9 us at 4096 x 4096 (1024 blocks), 10.3 / 10.0 us at 4096 -> 11008 (2752),
+// 38.9 / 34.1 us at 8192 -> 28672 (14336); 16 rows there: 76 / 59 us.
+constexpr int64_t kStreamBlocks = 4096;
+
+// CTAs per 128 rows of the streaming kernel: as many as give every SM three
+// (8192 -> 28672: 62 / 34 / 38 / 36 / 36 / 39 us for 1 / 2 / 3 / 4 / 5 / 8).
+int pick_stream_splits(const W4Args& a, int sm_count) {
+  const int64_t tiles = ceil_div(a.N, 128), blocks = ceil_div(a.K, 128);
+  int s = 1;
+  while (s < 8 && s * 4 <= blocks && tiles * s < 3 * sm_count) s *= 2;
+  return s;
+}
+
+template <class Cfg>
+int32_t launch_w4_stream(const W4Args& a, const DeviceInfo& dev, int device, cudaStream_t s) {
+  CUtensorMap mw, mx;
+  int32_t st = encode_words(&mw, a, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (st != SF_OK) return st;
+  const cuuint64_t dims[3] = {32, static_cast<cuuint64_t>(a.M), static_cast<cuuint64_t>(a.K / 32)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.ldx) * 2, 64};
+  const cuuint32_t box[3] = {32, 8 * Cfg::NT, 4};
+  st = encode(&mx, tma_dtype(a.dtype), a.x, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (st != SF_OK) return st;
+  const int64_t groups = ceil_div(a.K, 32 * Cfg::GW);
+  const cuuint64_t sdims[2] = {static_cast<cuuint64_t>(a.N), static_cast<cuuint64_t>(groups)};
+  const cuuint64_t sstrides[1] = {static_cast<cuuint64_t>(a.lds) * 2};
+  const cuuint32_t sbox[2] = {128, Cfg::NG};
+  CUtensorMap ms, mz;
+  st = encode(&ms, tma_dtype(a.dtype), a.scales, 2, sdims, sstrides, sbox, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (st == SF_OK)
+    st = encode(&mz, tma_dtype(a.dtype), a.zeros ? a.zeros : a.scales, 2, sdims, sstrides, sbox,
+                CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (st != SF_OK) return st;
+  static std::atomic<bool> allowed[64];
+  st = allow_smem(w4_stream_kernel<Cfg>, Cfg::SMEM_BYTES, device, allowed);
+  if (st != SF_OK) return st;
+  const int splits = pick_stream_splits(a, dev.sm_count);
+  return launch_cluster(w4_stream_kernel<Cfg>, ceil_div(a.N, 128) * splits, Cfg::THREADS, Cfg::SMEM_BYTES, splits, s,
+                        mw, mx, ms, mz, a, splits, dev.err_word);
+}
+
+template <bool BF16, int NT>
+int32_t launch_w4_stream_group(const W4Args& a, const DeviceInfo& dev, int device, cudaStream_t s) {
+  if (a.group == 32) return launch_w4_stream<W4StreamCfg<BF16, NT, 1>>(a, dev, device, s);
+  if (a.group == 64) return launch_w4_stream<W4StreamCfg<BF16, NT, 2>>(a, dev, device, s);
+  return launch_w4_stream<W4StreamCfg<BF16, NT, 4>>(a, dev, device, s);
 }
 
 // CTAs per row tile, which share its blocks.  A block takes a CTA about as long
@@ -325,60 +383,49 @@ int pick_w4_splits(const W4Args& a, int sm_count) {
 template <class Cfg>
 int32_t launch_w4_tc(const W4Args& a, const DeviceInfo& dev, int device, cudaStream_t s) {
   const int n_rows = (a.M + 15) / 16 * 16;
-  const int64_t blocks = ceil_div(a.K, 128);
   CUtensorMap mw, mx;
-  int32_t st = encode_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.packed, blocks * 16, a.N, a.ldp * 4, 16, 128,
-                         CU_TENSOR_MAP_SWIZZLE_64B);
-  if (st == SF_OK)
-    st = encode_2d(&mx, tma_dtype(a.dtype), a.x, a.K, a.M, a.ldx * 2, 64, n_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  int32_t st = encode_words(&mw, a, CU_TENSOR_MAP_SWIZZLE_64B);
   if (st != SF_OK) return st;
-  if (device >= 64) return fail(SF_ERR_UNSUPPORTED, "device index %d", device);
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.K), static_cast<cuuint64_t>(a.M)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.ldx) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(n_rows)};
+  st = encode(&mx, tma_dtype(a.dtype), a.x, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != SF_OK) return st;
   static std::atomic<bool> allowed[64];
-  if (!allowed[device].load(std::memory_order_acquire)) {
-    SF_CUDA_TRY(cudaFuncSetAttribute(w4_tc_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     Cfg::SMEM_BYTES));
-    allowed[device].store(true, std::memory_order_release);
-  }
+  st = allow_smem(w4_tc_kernel<Cfg>, Cfg::SMEM_BYTES, device, allowed);
+  if (st != SF_OK) return st;
   const int splits = pick_w4_splits(a, dev.sm_count);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(a.N, 128) * splits));
-  cfg.blockDim = dim3(Cfg::THREADS);
-  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  SF_CUDA_TRY(cudaLaunchKernelEx(&cfg, w4_tc_kernel<Cfg>, mw, mx, a, splits, n_rows, dev.err_word));
-  return SF_OK;
+  return launch_cluster(w4_tc_kernel<Cfg>, ceil_div(a.N, 128) * splits, Cfg::THREADS, Cfg::SMEM_BYTES, splits, s, mw,
+                        mx, a, splits, n_rows, dev.err_word);
 }
 
-// Up to 16 rows of x run on mma.sync, more on tcgen05 (16 rows: 7.5 against 8.9
-// us at 4096 x 4096, 76 against 68 us at 8192 -> 28672; 33 rows: 213 against 69
-// us there).  Rows of x that TMA cannot describe take the former, 16 at a time.
+// Up to 16 rows of x run on mma.sync, more on tcgen05 (33 rows: 71 us at 8192 ->
+// 28672, 213 in three passes of the ring kernel).  Rows of x that TMA cannot
+// describe take the ring kernel.
 template <bool BF16>
 int32_t run_w4(const W4Args& a, cudaStream_t s) {
-  if (a.M > 16 && a.ldx % 8 == 0 && aligned16(a.x)) {
-    DeviceInfo* dev = nullptr;
-    int device = 0;
-    const int32_t st = current_device_info(&dev, &device);
-    if (st != SF_OK) return st;
+  const bool described = a.ldx % 8 == 0 && aligned16(a.x);
+  DeviceInfo* dev = nullptr;
+  int device = 0;
+  int32_t st = current_device_info(&dev, &device);
+  if (st != SF_OK) return st;
+  if (described && a.M <= 16 && a.K % 32 == 0 && a.lds % 8 == 0 && aligned16(a.scales) && aligned16(a.zeros) &&
+      ceil_div(a.N, 128) * ceil_div(a.K, 128) >= kStreamBlocks)
+    return a.M <= 8 ? launch_w4_stream_group<BF16, 1>(a, *dev, device, s)
+                    : launch_w4_stream_group<BF16, 2>(a, *dev, device, s);
+  if (described && a.M > 16 && a.K > 0) {
     if (a.group == 32) return launch_w4_tc<W4TcCfg<BF16, 1>>(a, *dev, device, s);
     if (a.group == 64) return launch_w4_tc<W4TcCfg<BF16, 2>>(a, *dev, device, s);
     return launch_w4_tc<W4TcCfg<BF16, 4>>(a, *dev, device, s);
   }
-  const bool x_vec = a.K % 8 == 0 && a.ldx % 8 == 0 && aligned16(a.x);
+  const bool x_vec = a.K % 8 == 0 && described;
   if (a.M <= 8) return launch_w4_group<BF16, 1>(a, x_vec, s);
   W4Args p = a;
   for (int m0 = 0; m0 < a.M; m0 += 16) {
     p.M = std::min(16, a.M - m0);
     p.x = static_cast<const uint16_t*>(a.x) + m0 * a.ldx;
     p.y = static_cast<char*>(a.y) + m0 * a.ldy * esize(a.out_dtype);
-    const int32_t st = launch_w4_group<BF16, 2>(p, x_vec, s);
+    st = launch_w4_group<BF16, 2>(p, x_vec, s);
     if (st != SF_OK) return st;
   }
   return SF_OK;

@@ -236,11 +236,11 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2)
       const uint32_t sw64 = (row >> 1) & 3;
       int stage = 0, ab = 0;
       uint32_t phase = 0, aphase = 0;
-      uint16_t zn[2][NG];  // two blocks ahead
-      auto load_zeros = [&](uint16_t (&to)[NG], int b) {
+      uint32_t zn[2][NG];  // two blocks ahead
+      auto load_zeros = [&](uint32_t (&to)[NG], int b) {
+        if (!zeros) return;
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-          to[g] = zeros && b < b1 && b * NG + g < groups ? __ldg(zp + (b * NG + g) * a.lds) : 0;
+        for (int g = 0; g < NG; ++g) to[g] = load_ahead(zp + min(b * NG + g, groups - 1) * a.lds);
       };
       load_zeros(zn[0], b0);
       load_zeros(zn[1], b0 + 1);
@@ -299,13 +299,11 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2)
 #pragma unroll
       for (int i = 0; i < SC; ++i) acc[i] = 0.0f;
       const uint16_t* sp = static_cast<const uint16_t*>(a.scales) + n;
-      auto scale = [&](int grp) -> uint16_t {
-        return grp < min(groups, b1 * NG) ? __ldg(sp + grp * a.lds) : 0;
-      };
+      auto scale = [&](int grp) { return load_ahead(sp + min(grp, groups - 1) * a.lds); };
       int db = 0;
       uint32_t dphase = 0;
       constexpr int AHEAD = 4;  // groups
-      uint16_t next[AHEAD];
+      uint32_t next[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) next[i] = scale(b0 * NG + i);
       bool ok = true;
@@ -313,8 +311,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2)
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           if (g0 + i >= b1 * NG) break;
-          const float s = Cfg::BF16 ? __uint_as_float(static_cast<uint32_t>(next[i]) << 16)
-                                    : __half2float(__ushort_as_half(next[i]));
+          const float s = g0 + i < groups ? w4_float<Cfg::BF16>(next[i]) : 0.0f;
           next[i] = scale(g0 + i + AHEAD);
           ok = mbar_wait(&dfull_bar[db], dphase, err, kDevTimeoutEpilogue, abortp);
           if (!ok) break;

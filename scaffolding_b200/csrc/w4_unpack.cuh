@@ -43,6 +43,12 @@ __device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t m
 // A stored zero point as the whole number 0..15 it stands for.
 __device__ __forceinline__ float whole_zero(float z) { return fminf(fmaxf(rintf(z), 0.0f), 15.0f); }
 
+// fp32 value of 16 stored bits.
+template <bool BF16>
+__device__ __forceinline__ float w4_float(uint32_t v) {
+  return BF16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(v)));
+}
+
 // Word -> four pairs (columns 2 i, 2 i + 1) of q - z.  z is the pair constant
 // of the group: 128 + z (bf16); 1024 + z in .x and 64 + z in .y (fp16).
 template <bool BF16>
@@ -72,12 +78,21 @@ __device__ __forceinline__ void unpack_word(uint32_t w, uint2 z, uint32_t (&p)[4
   }
 }
 
+// A scale or zero point ahead of its use.  A register of its own for each, and
+// no branch or select on the value: either would make the load be waited for
+// where it is issued (250 cycles each, measured).
+__device__ __forceinline__ uint32_t load_ahead(const uint16_t* p) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .u16 t;\n\tld.global.nc.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(v) : "l"(p));
+  return v;
+}
+
 // The pair constant of a stored zero point (16 bits, low half of v): adding
 // the magic rounds it to a whole number, the clamp keeps it in 0..15 (a NaN
 // becomes 0), as whole_zero does.
 template <bool BF16>
-__device__ __forceinline__ uint2 zero_pair(uint16_t v) {
-  const uint32_t two = static_cast<uint32_t>(v) * 0x10001u;
+__device__ __forceinline__ uint2 zero_pair(uint32_t v) {
+  const uint32_t two = v * 0x10001u;
   uint2 r;
   if constexpr (BF16) {
     __nv_bfloat162 m = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&two), __float2bfloat162_rn(128.0f));
@@ -92,6 +107,34 @@ __device__ __forceinline__ uint2 zero_pair(uint16_t v) {
     r.y = *reinterpret_cast<const uint32_t*>(&n);
   }
   return r;
+}
+
+// Accumulators of one 16 x 8 tile and group.  An mma.sync that adds to the result
+// of the one before it waits about 140 cycles for it (a block of eight chained
+// ones took 1100 cycles, in two chains of four 534), so a group's mmas go round
+// several accumulators, as many as there are registers for.
+__host__ __device__ constexpr int w4_accumulators(int nt, int gw) { return nt == 1 && gw > 1 ? 4 : 2; }
+
+template <int NA>
+__device__ __forceinline__ float sum_of(const float (&s)[NA][4], int c) {
+  return NA == 4 ? (s[0][c] + s[1][c]) + (s[NA - 2][c] + s[NA - 1][c]) : s[0][c] + s[1][c];
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 }  // namespace sf
