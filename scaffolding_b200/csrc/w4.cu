@@ -28,6 +28,38 @@
 namespace sf {
 namespace {
 
+// A launch in clusters of `splits` CTAs with programmatic stream serialisation.
+template <class Kernel, class... Args>
+int32_t launch_cluster(Kernel kernel, int64_t grid, int threads, size_t smem, int splits, cudaStream_t s,
+                       Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  SF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+  return SF_OK;
+}
+
+// The opt-in to a kernel's dynamic shared memory, once per device.
+template <class Kernel>
+int32_t allow_smem(Kernel kernel, int bytes, int device, std::atomic<bool> (&allowed)[64]) {
+  if (device >= 64) return fail(SF_ERR_UNSUPPORTED, "device index %d", device);
+  if (!allowed[device].load(std::memory_order_acquire)) {
+    SF_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    allowed[device].store(true, std::memory_order_release);
+  }
+  return SF_OK;
+}
+
 // ───────────────────────── ring kernel ─────────────────────────
 // Up to 16 rows of x, any layout: the unpacking and the fragments of
 // w4_stream.cuh with less around them.  A warp owns 32 weight rows and every
@@ -36,7 +68,6 @@ namespace {
 // per lane.  The WK partial sums of a row meet in shared memory, in warp order.
 // More than 16 rows of x run in passes of 16.
 
-constexpr int kW4Threads = 256;
 constexpr int kW4Rows = 32;   // weight rows of a warp
 constexpr int kW4Stages = 3;  // blocks in flight per warp
 
@@ -65,8 +96,8 @@ __device__ __forceinline__ void copy_async_wait() {
 }
 
 // GW: 32-column words per group (1, 2, 4).
-template <bool BF16, int NT, int GW>
-__global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int wk, int x_vec) {
+template <bool BF16, int NT, int GW, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) w4_mma_kernel(const W4Args a, int wk, int x_vec) {
   constexpr int NG = 4 / GW;             // groups per block
   constexpr int NA = w4_accumulators(NT, GW);
   constexpr int kSlot = (4 + 4 * NT) * 32;  // 16-byte vectors per block: a lane's words and x
@@ -134,6 +165,8 @@ __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int 
     }
     ++scaled;
   };
+  pdl_launch_dependents();
+  pdl_wait();
   load_scales(0);
   load_scales(1);
   for (int i = 0; i < kW4Stages - 1; ++i) copy_block(i);
@@ -226,30 +259,39 @@ __global__ void __launch_bounds__(kW4Threads) w4_mma_kernel(const W4Args a, int 
   }
 }
 
-template <bool BF16, int NT, int GW>
-int32_t launch_w4(const W4Args& a, bool x_vec, cudaStream_t s) {
+template <bool BF16, int NT, int GW, int WARPS>
+int32_t launch_w4(const W4Args& a, bool x_vec, int device, cudaStream_t s) {
   // Warps along k: as many as there are blocks for, so that every row's
   // stream is spread over the CTA; the rest take further rows.
   const int64_t blocks = ceil_div(a.K, 128);
-  constexpr int warps = kW4Threads / 32;
   int wk = 1;
-  while (wk < warps && wk < blocks) wk *= 2;
-  const int64_t rows = kW4Rows * (warps / wk);
-  const size_t smem = static_cast<size_t>(warps) *
-                      std::max(kW4Stages * (4 + 4 * NT) * 32 * 16, kW4Rows * 8 * NT * static_cast<int>(sizeof(float)));
-  SF_CUDA_TRY(cudaFuncSetAttribute(w4_mma_kernel<BF16, NT, GW>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  w4_mma_kernel<BF16, NT, GW>
-      <<<static_cast<unsigned>(ceil_div(a.N, rows)), warps * 32, smem, s>>>(a, wk, x_vec ? 1 : 0);
-  SF_CUDA_TRY(cudaGetLastError());
-  return SF_OK;
+  while (wk < WARPS && wk < blocks) wk *= 2;
+  const int64_t rows = kW4Rows * (WARPS / wk);
+  constexpr int smem =
+      WARPS * std::max(kW4Stages * (4 + 4 * NT) * 32 * 16, kW4Rows * 8 * NT * static_cast<int>(sizeof(float)));
+  static std::atomic<bool> allowed[64];
+  const int32_t st = allow_smem(w4_mma_kernel<BF16, NT, GW, WARPS>, smem, device, allowed);
+  if (st != SF_OK) return st;
+  return launch_cluster(w4_mma_kernel<BF16, NT, GW, WARPS>, ceil_div(a.N, rows), 32 * WARPS, smem, 1, s, a, wk,
+                        x_vec ? 1 : 0);
 }
 
+// Sixteen warps per CTA where 32-row tiles are no more than the SMs: 4.4 against
+// 6.5 us (1 x 4096 x 4096), 13 against 21 us (8 x 11008 -> 4096, groups of 32).
+// With eight, two CTAs fit an SM, and the next launch's, which start early, then
+// pair up on some SMs while others stay empty.
 template <bool BF16, int NT>
-int32_t launch_w4_group(const W4Args& a, bool x_vec, cudaStream_t s) {
-  if (a.group == 32) return launch_w4<BF16, NT, 1>(a, x_vec, s);
-  if (a.group == 64) return launch_w4<BF16, NT, 2>(a, x_vec, s);
-  return launch_w4<BF16, NT, 4>(a, x_vec, s);
+int32_t launch_w4_group(const W4Args& a, bool x_vec, const DeviceInfo& dev, int device, cudaStream_t s) {
+  if constexpr (NT == 1) {
+    if (ceil_div(a.N, kW4Rows) <= dev.sm_count && a.K > 8 * 128) {
+      if (a.group == 32) return launch_w4<BF16, NT, 1, 16>(a, x_vec, device, s);
+      if (a.group == 64) return launch_w4<BF16, NT, 2, 16>(a, x_vec, device, s);
+      return launch_w4<BF16, NT, 4, 16>(a, x_vec, device, s);
+    }
+  }
+  if (a.group == 32) return launch_w4<BF16, NT, 1, 8>(a, x_vec, device, s);
+  if (a.group == 64) return launch_w4<BF16, NT, 2, 8>(a, x_vec, device, s);
+  return launch_w4<BF16, NT, 4, 8>(a, x_vec, device, s);
 }
 
 // ───────────────────────── tcgen05 kernel ─────────────────────────
@@ -275,38 +317,6 @@ int32_t encode_words(CUtensorMap* m, const W4Args& a, CUtensorMapSwizzle swizzle
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.ldp) * 4};
   const cuuint32_t box[2] = {16, 128};
   return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.packed, 2, dims, strides, box, swizzle);
-}
-
-// A launch in clusters of `splits` CTAs with programmatic stream serialisation.
-template <class Kernel, class... Args>
-int32_t launch_cluster(Kernel kernel, int64_t grid, int threads, size_t smem, int splits, cudaStream_t s,
-                       Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  SF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
-  return SF_OK;
-}
-
-// The opt-in to a kernel's dynamic shared memory, once per device.
-template <class Kernel>
-int32_t allow_smem(Kernel kernel, int bytes, int device, std::atomic<bool> (&allowed)[64]) {
-  if (device >= 64) return fail(SF_ERR_UNSUPPORTED, "device index %d", device);
-  if (!allowed[device].load(std::memory_order_acquire)) {
-    SF_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    allowed[device].store(true, std::memory_order_release);
-  }
-  return SF_OK;
 }
 
 // Blocks of 128 x 128 from which the streaming kernel is used.  Its clusters and
@@ -419,13 +429,13 @@ int32_t run_w4(const W4Args& a, cudaStream_t s) {
     return launch_w4_tc<W4TcCfg<BF16, 4>>(a, *dev, device, s);
   }
   const bool x_vec = a.K % 8 == 0 && described;
-  if (a.M <= 8) return launch_w4_group<BF16, 1>(a, x_vec, s);
+  if (a.M <= 8) return launch_w4_group<BF16, 1>(a, x_vec, *dev, device, s);
   W4Args p = a;
   for (int m0 = 0; m0 < a.M; m0 += 16) {
     p.M = std::min(16, a.M - m0);
     p.x = static_cast<const uint16_t*>(a.x) + m0 * a.ldx;
     p.y = static_cast<char*>(a.y) + m0 * a.ldy * esize(a.out_dtype);
-    st = launch_w4_group<BF16, 2>(p, x_vec, s);
+    st = launch_w4_group<BF16, 2>(p, x_vec, *dev, device, s);
     if (st != SF_OK) return st;
   }
   return SF_OK;

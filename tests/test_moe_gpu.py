@@ -237,6 +237,32 @@ def test_grouped_every_row_in_one_group_and_long_groups(gpu, ops, dt):
         assert_within(*run_grouped(ops, rng, dt, X, M, 256, 320, "gelu_tanh", True, offsets=offsets))
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_grouped_rows_gathered_first(gpu, ops, dt):
+    """Long batches copy their rows into grouped order first (outside a
+    capture): the same bits as the rows given in that order, zeros for an
+    index outside x, a width that ends inside a 16-byte vector."""
+    from scaffolding_b200 import engine as E
+    rng = np.random.default_rng(21)
+    X, M, K, N, T = 6, 2500, 200, 1030, 900
+    gx, x = to_device(ops, rng.standard_normal((T, K), dtype=np.float32), dt)
+    gw, w = to_device(ops, rng.uniform(-1, 1, (X, N, K)).astype(np.float32) / np.float32(14), dt)
+    rows = rng.integers(0, T, M).astype(np.int32)
+    rows[[0, 77, 2499]] = [-1, T, 2 ** 31 - 1]
+    offsets = groups_of(rng, M, X, empty=(2,))
+    need = C.c_size_t()
+    assert E.lib.sf_gemm_grouped_workspace_size(X, M, N, K, E.dtype_code(np_dtype(dt)), None, C.byref(need)) == 0
+    assert need.value == M * K * 2
+    go = ops.gputensor_from_numpy(offsets)
+    y = to_host32(ops, ops.dev_grouped_linear(gx, gw, go, rows=ops.gputensor_from_numpy(rows)))
+    ref, tol = plain_grouped(x, w, offsets, None, "none", rows, dt)
+    assert_within(y.astype(np.float64), ref, tol)
+    dense = np.stack([x[r] if 0 <= r < T else np.zeros(K, np.float32) for r in rows])
+    gd, _ = to_device(ops, dense, dt)
+    assert np.array_equal(y, to_host32(ops, ops.dev_grouped_linear(gd, gw, go)))
+    assert device_error(0) == 0
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_grouped_rows_outside(gpu, ops, dt):
     """Rows in no group keep what they held, indices outside x read zeros and

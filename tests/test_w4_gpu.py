@@ -97,6 +97,16 @@ def test_linear_wide(gpu, ops, dt):
     run(ops, rng, dt, 64, 700, 4224, 64, False)
 
 
+@pytest.mark.parametrize("dt,group,zeros", [("bf16", 128, False), ("f16", 32, True), ("bf16", 64, True)])
+@pytest.mark.parametrize("M", [1, 5, 16])
+def test_linear_streamed(gpu, ops, dt, group, zeros, M):
+    """Sizes of the streaming kernel (4096 blocks of 128 x 128 and more, up to
+    16 rows): a last tile of 8 rows, a last block cut short, clusters of two."""
+    rng = np.random.default_rng(M)
+    run(ops, rng, dt, M, 16392, 4064, group, zeros, "silu", True)
+    assert device_error(0) == 0
+
+
 @pytest.mark.parametrize("M", [1, 9])
 def test_linear_large_values(gpu, ops, M):
     """x at the edge of fp16's range: group sums stay in fp32."""
