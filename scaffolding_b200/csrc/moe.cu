@@ -342,7 +342,7 @@ int route_chunk(int64_t tokens) {
 // adds nothing.  Bound by HBM: every expert row is read once (the slots of
 // all choices are a permutation) and every output row written once, so each
 // thread owns 16 bytes of an output row and has the loads of up to four expert
-// rows in flight.  Measured at 17776 x 1920 bf16, two experts: 42.4 us, 4.84
+// rows in flight.  Measured at 17776 x 1920 bf16, two experts: 40.9 us, 5.01
 // TB/s of 6.53.
 
 struct CombineArgs {
@@ -396,58 +396,80 @@ __device__ __forceinline__ void unpack_vec(const uint4& u, float* f) {
   }
 }
 
-// 16 bytes of an output row per thread; KK rows of y are in flight at once (the
-// last KK - top_k % KK of a token read nothing).
-template <int DT, int KK>
+// UU x 16 bytes of the output per thread, 256 vectors apart; KK rows of y of each
+// are in flight at once (the last KK - top_k % KK of a token read nothing).
+template <int DT, int KK, int UU>
 __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineArgs a) {
   constexpr int E = DT == kF32 ? 4 : 8, ES = DT == kF32 ? 4 : 2;
   pdl_launch_dependents();
   const int vecs = a.cols / E;
-  const int64_t i = blockIdx.x * 256LL + threadIdx.x;
-  const int64_t t = i / vecs;
-  const int c = static_cast<int>(i - t * vecs) * E;
-  pdl_wait();
-  if (t >= a.tokens) return;
-  float acc[E] = {};
-  if (a.residual)
-    unpack_vec<DT>(*reinterpret_cast<const uint4*>(static_cast<const char*>(a.residual) + (t * a.ldr + c) * ES), acc);
-  const int* slots = a.slots + t * a.k;
-  const float* weights = a.weights + t * a.k;
-  for (int j0 = 0; j0 < a.k; j0 += KK) {
-    uint4 u[KK];
-    float w[KK];
-    bool live[KK];
+  const int64_t i0 = blockIdx.x * (256LL * UU) + threadIdx.x;
+  int64_t t[UU];
+  int c[UU];
 #pragma unroll
-    for (int j = 0; j < KK; ++j) {
-      const int64_t s = j0 + j < a.k ? slots[j0 + j] : -1;
-      live[j] = s >= 0 && s < a.y_rows;
-      w[j] = live[j] ? weights[j0 + j] : 0.0f;
-      if (live[j])
-        u[j] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const char*>(a.y) + (s * a.ldy + c) * ES));
-    }
-#pragma unroll
-    for (int j = 0; j < KK; ++j)
-      if (live[j]) {
-        float f[E];
-        unpack_vec<DT>(u[j], f);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(w[j], f[e], acc[e]);
-      }
+  for (int u = 0; u < UU; ++u) {
+    const int64_t i = i0 + 256 * u;
+    t[u] = i <= UINT_MAX ? static_cast<uint32_t>(i) / static_cast<uint32_t>(vecs) : i / vecs;
+    c[u] = static_cast<int>(i - t[u] * vecs) * E;
   }
-  char* o = static_cast<char*>(a.out) + (t * a.ldo + c) * ES;
-  if constexpr (DT == kF32)
-    *reinterpret_cast<float4*>(o) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  else
-    *reinterpret_cast<uint4*>(o) = make_uint4(pack2(acc[0], acc[1], DT), pack2(acc[2], acc[3], DT),
-                                              pack2(acc[4], acc[5], DT), pack2(acc[6], acc[7], DT));
+  pdl_wait();
+  float acc[UU][E] = {};
+  if (a.residual)
+#pragma unroll
+    for (int u = 0; u < UU; ++u)
+      if (t[u] < a.tokens)
+        unpack_vec<DT>(*reinterpret_cast<const uint4*>(static_cast<const char*>(a.residual) + (t[u] * a.ldr + c[u]) * ES),
+                       acc[u]);
+  for (int j0 = 0; j0 < a.k; j0 += KK) {
+    uint4 v[UU][KK];
+    float w[UU][KK];
+    bool live[UU][KK];
+#pragma unroll
+    for (int u = 0; u < UU; ++u)
+#pragma unroll
+      for (int j = 0; j < KK; ++j) {
+        const bool in = t[u] < a.tokens && j0 + j < a.k;
+        const int64_t s = in ? a.slots[t[u] * a.k + j0 + j] : -1;
+        live[u][j] = s >= 0 && s < a.y_rows;
+        w[u][j] = live[u][j] ? a.weights[t[u] * a.k + j0 + j] : 0.0f;
+        if (live[u][j])
+          v[u][j] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const char*>(a.y) + (s * a.ldy + c[u]) * ES));
+      }
+#pragma unroll
+    for (int u = 0; u < UU; ++u)
+#pragma unroll
+      for (int j = 0; j < KK; ++j)
+        if (live[u][j]) {
+          float f[E];
+          unpack_vec<DT>(v[u][j], f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[u][e] = fmaf(w[u][j], f[e], acc[u][e]);
+        }
+  }
+#pragma unroll
+  for (int u = 0; u < UU; ++u) {
+    if (t[u] >= a.tokens) break;
+    char* o = static_cast<char*>(a.out) + (t[u] * a.ldo + c[u]) * ES;
+    const float(&f)[E] = acc[u];
+    if constexpr (DT == kF32)
+      *reinterpret_cast<float4*>(o) = make_float4(f[0], f[1], f[2], f[3]);
+    else
+      *reinterpret_cast<uint4*>(o) = make_uint4(pack2(f[0], f[1], DT), pack2(f[2], f[3], DT), pack2(f[4], f[5], DT),
+                                                pack2(f[6], f[7], DT));
+  }
 }
 
 template <int DT>
 int32_t launch_combine_vec(const CombineArgs& a, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>(ceil_div(a.tokens * (a.cols / (DT == kF32 ? 4 : 8)), 256));
-  if (a.k <= 1) return launch_pdl(combine_vec_kernel<DT, 1>, grid, 256, 0, s, a);
-  if (a.k <= 2) return launch_pdl(combine_vec_kernel<DT, 2>, grid, 256, 0, s, a);
-  return launch_pdl(combine_vec_kernel<DT, 4>, grid, 256, 0, s, a);
+  const int64_t vecs = a.tokens * (a.cols / (DT == kF32 ? 4 : 8));
+  // Two vectors per thread where one leaves few loads in flight (us at 1920
+  // columns, one / two vectors: 17776 tokens bf16, top 1 36 / 29, top 2 42 / 41;
+  // 8000 tokens, top 4 32 / 39, fp32 top 2 37 / 39).
+  const unsigned two = static_cast<unsigned>(ceil_div(vecs, 512)), one = static_cast<unsigned>(ceil_div(vecs, 256));
+  if (a.k == 1) return launch_pdl(combine_vec_kernel<DT, 1, 2>, two, 256, 0, s, a);
+  if (a.k == 2 && DT != kF32) return launch_pdl(combine_vec_kernel<DT, 2, 2>, two, 256, 0, s, a);
+  if (a.k == 2) return launch_pdl(combine_vec_kernel<DT, 2, 1>, one, 256, 0, s, a);
+  return launch_pdl(combine_vec_kernel<DT, 4, 1>, one, 256, 0, s, a);
 }
 
 bool known_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
