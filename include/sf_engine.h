@@ -169,7 +169,8 @@ int32_t sf_linear_skinny_noalloc(int64_t M, int64_t N, int64_t K,
  * offsets are clamped to 0..M and to their running maximum.
  *   B [groups][N][K] in the nn.Linear layout ([groups][2 N][K] for
  *   SF_ACT_SILU_GATE: N gate rows, then N value rows), rows ldb apart and
- *   groups b_stride apart; bias likewise, bias_stride apart, or NULL.
+ *   groups b_stride apart (0: one weight for all); bias likewise, bias_stride
+ *   apart, or NULL.  C shares no memory with the inputs.
  * 16-bit operands whose rows start on 16-byte boundaries run on the tensor
  * cores; fp32 and other layouts on the FMA pipe (IEEE fp32).  At most 4096
  * groups.  The workspace is optional: with
@@ -408,6 +409,9 @@ int32_t sf_graph_begin(void* stream);
 int32_t sf_graph_end(void* stream, void** exec);
 int32_t sf_graph_launch(void* exec, void* stream);
 int32_t sf_graph_destroy(void* exec);
+/* *capturing = 1 while work on `stream` is being captured, or (the legacy
+ * stream) would be refused because another stream is. */
+int32_t sf_stream_is_capturing(void* stream, int32_t* capturing);
 
 /* Peer access (_cuda_ops.pyx:550-587). */
 int32_t sf_can_access_peer(int32_t device, int32_t peer, int32_t* can);

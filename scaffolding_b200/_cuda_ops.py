@@ -429,6 +429,12 @@ def _result(out, shape, dtype, dev, name: str) -> GpuTensor:
     return out
 
 
+def _apart(out, *inputs) -> None:
+    """Refuses a result buffer that is an input's."""
+    if out is not None and out.numel and any(t is not None and t.buffer is out.buffer for t in inputs):
+        raise ValueError("out must not share memory with the inputs")
+
+
 def _int32(t: GpuTensor, name: str) -> GpuTensor:
     if t.dtype != _I32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
@@ -530,6 +536,7 @@ def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTen
     N = wide // 2 if act == ACT_SILU_GATE else wide
     M = rows.shape[0] if rows is not None else gt_x.shape[0]
     dev = _same_device(gt_x, gt_weight, gt_offsets, gt_bias, rows, out)
+    _apart(out, gt_x, gt_weight, gt_bias)
     odt = _out_dtype(gt_x, out_dtype if out is None else out.dtype)
     y = _result(out, (M, N), odt, dev, "out")
     bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
@@ -556,7 +563,8 @@ def dev_moe_combine(gt_y: GpuTensor, gt_slots: GpuTensor, gt_weights: GpuTensor,
     """Weighted sum of every token's expert rows (``sf_moe_combine``):
     ``residual[t] + sum_j weights[t, j] * y[slots[t, j]]`` in fp32, rounded
     once; ``slots`` and ``weights`` as in a MoeRoute, ``y`` ``[slots, C]``.
-    A slot outside ``y`` (-1, say, for a dropped choice) adds nothing."""
+    A slot outside ``y`` (-1, say, for a dropped choice) adds nothing.  ``out``
+    may be ``residual``, not ``y``."""
     if gt_y.ndim != 2 or gt_slots.ndim != 2:
         raise ValueError(f"combine shapes: y {gt_y.shape}, slots {gt_slots.shape}")
     T, k = _int32(gt_slots, "slots").shape
@@ -566,6 +574,7 @@ def dev_moe_combine(gt_y: GpuTensor, gt_slots: GpuTensor, gt_weights: GpuTensor,
     if residual is not None and (residual.shape != (T, width) or residual.dtype != gt_y.dtype):
         raise ValueError(f"residual must be {(T, width)} {gt_y.dtype}, got {residual.shape} {residual.dtype}")
     dev = _same_device(gt_y, gt_slots, gt_weights, residual, out)
+    _apart(out, gt_y)
     o = _result(out, (T, width), gt_y.dtype, dev, "out")
     with E.on_device(dev):
         check(lib.sf_moe_combine(T, width, k, _ptr(gt_y), gt_y.shape[0], width,
@@ -613,6 +622,8 @@ class W4Weight:
                  in_features: int, group: int = 128):
         if group not in (32, 64, 128):
             raise ValueError(f"group of {group} columns (32, 64 or 128)")
+        if in_features < 1:
+            raise ValueError(f"a 4-bit weight of {in_features} columns")
         if packed.ndim != 2 or packed.dtype not in (_U32, _I32):
             raise ValueError(f"packed must be 2-d uint32, got {packed.shape} {packed.dtype}")
         n = packed.shape[0]
@@ -697,9 +708,12 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
                   activation: str = "none", out_dtype=None, out: GpuTensor | None = None) -> GpuTensor:
     """``dev_linear_forward`` over a 4-bit weight: ``act(x @ W^T + bias)`` for
     bf16 / fp16 x.  Up to 64 rows of x run on ``sf_linear_w4``, which streams
-    the packed weight once; more rows dequantise it into a 16-bit weight (one
-    more rounding per weight, which the streamed product does not make) and
-    run the GEMM."""
+    the packed weight; more rows dequantise it into a 16-bit weight (one more
+    rounding per weight, which the streamed product does not make) and run
+    the GEMM.  During a graph capture more rows run 64 at a time on
+    ``sf_linear_w4`` instead: a graph must not hold the dequantised weight,
+    whose memory is free again when the call returns.  ``out`` shares no
+    memory with x."""
     act = E.act_code(activation)
     if gt_x.dtype != weight.scales.dtype:
         raise TypeError(f"x and the weight's scales must share a dtype ({gt_x.dtype} vs {weight.scales.dtype})")
@@ -712,16 +726,21 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
         raise ValueError(f"bias has {gt_bias.numel} elements, expected {n}")
     M = int(math.prod(gt_x.shape[:-1]))
     dev = _same_device(gt_x, weight.packed, gt_bias, out)
+    _apart(out, gt_x, gt_bias)
     odt = _out_dtype(gt_x, out_dtype if out is None else out.dtype)
     y = _result(out, gt_x.shape[:-1] + (n,), odt, dev, "out")
     bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
     in_code, out_code = E.dtype_code(gt_x.dtype), E.dtype_code(odt)
+    stream = E.get_stream(dev)
     with E.on_device(dev):
-        if M <= _W4_MAX_ROWS:
-            check(lib.sf_linear_w4(M, n, k, _ptr(gt_x), k, _ptr(weight.packed),
-                                   weight.packed.shape[1], _ptr(weight.scales), _ptr(weight.zeros),
-                                   n, weight.group, _ptr(gt_bias), bias_dt, _ptr(y), n, in_code,
-                                   out_code, act, E.get_stream(dev)), "sf_linear_w4")
+        if M <= _W4_MAX_ROWS or E.stream_capturing(stream):
+            x_row, y_row = k * gt_x.dtype.itemsize, n * odt.itemsize
+            for m0 in range(0, M, _W4_MAX_ROWS):
+                check(lib.sf_linear_w4(min(M - m0, _W4_MAX_ROWS), n, k, gt_x.ptr + m0 * x_row, k,
+                                       _ptr(weight.packed), weight.packed.shape[1],
+                                       _ptr(weight.scales), _ptr(weight.zeros), n, weight.group,
+                                       _ptr(gt_bias), bias_dt, y.ptr + m0 * y_row, n, in_code,
+                                       out_code, act, stream), "sf_linear_w4")
         else:
             w = dev_dequantize_w4(weight)
             epi = E.make_epilogue(bias_ptr=gt_bias.ptr if gt_bias is not None else 0,

@@ -212,14 +212,17 @@ extern "C" int32_t sf_gemm_grouped(int64_t groups, int64_t M, int64_t N, int64_t
       return fail(SF_ERR_INVALID_ARGUMENT, "unknown dtype %d", dt);
   if (groups == 0 || M == 0 || N == 0) return SF_OK;
   const int64_t wide = activation == SF_ACT_SILU_GATE ? 2 * N : N;
-  if (M > INT32_MAX || wide > INT32_MAX || K > INT32_MAX || a_rows > INT32_MAX)
-    return fail(SF_ERR_UNSUPPORTED, "dimension exceeds 2^31-1");
+  // Row and column counts are rounded up to tiles in 32 bits.
+  constexpr int64_t kMostRows = INT32_MAX - 4096;
+  if (M > kMostRows || wide > kMostRows || K > kMostRows || a_rows > INT32_MAX)
+    return fail(SF_ERR_UNSUPPORTED, "dimension exceeds 2^31-4097");
   if (groups > kMaxGroups)
     return fail(SF_ERR_UNSUPPORTED, "%lld groups (at most %lld)", (long long)groups, (long long)kMaxGroups);
   if (!offsets || !C || (K > 0 && (!A || !B))) return fail(SF_ERR_INVALID_ARGUMENT, "null pointer");
   if (!rows && a_rows < M)
     return fail(SF_ERR_INVALID_ARGUMENT, "A has %lld rows, %lld needed", (long long)a_rows, (long long)M);
   if (ldc < N || lda < K || ldb < K) return fail(SF_ERR_INVALID_ARGUMENT, "leading dimension too small");
+  if (b_stride < 0 || bias_stride < 0) return fail(SF_ERR_INVALID_ARGUMENT, "negative group stride");
   if (bias && bias_dtype != kF32 && bias_dtype != kF16 && bias_dtype != kBF16)
     return fail(SF_ERR_INVALID_ARGUMENT, "unknown bias dtype");
   DeviceInfo* dev = nullptr;
@@ -251,8 +254,8 @@ extern "C" int32_t sf_gemm_grouped(int64_t groups, int64_t M, int64_t N, int64_t
   a.err = dev->err_word;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool describable = in_dtype != kF32 && K > 0 && a_rows > 0 && aligned16(A) && aligned16(B) &&
-                           bytes16(lda, 2) && bytes16(ldb, 2) && (groups == 1 || bytes16(b_stride, 2)) &&
-                           b_stride >= 0;
+                           bytes16(lda, 2) && bytes16(ldb, 2) &&
+                           (groups == 1 || (b_stride > 0 && bytes16(b_stride, 2)));
   if (!describable) return run_simt(a, s);
   const size_t gathered = static_cast<size_t>(M) * static_cast<size_t>(gathered_ld(K)) * 2;
   if (rows && gather_pays(groups, M, N) && workspace && aligned16(workspace) && workspace_bytes >= gathered) {
@@ -268,12 +271,10 @@ extern "C" int32_t sf_gemm_grouped_workspace_size(int64_t groups, int64_t M, int
   *bytes = 0;
   if (groups < 0 || M < 0 || N < 0 || K < 0) return fail(SF_ERR_INVALID_ARGUMENT, "negative dimension");
   if (in_dtype == kF32 || K == 0 || !gather_pays(groups, M, N)) return SF_OK;
-  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capturing) != cudaSuccess) {
-    cudaGetLastError();  // the legacy stream while another one is captured
-    return SF_OK;
-  }
-  if (capturing == cudaStreamCaptureStatusNone)
+  int32_t capturing = 0;
+  const int32_t st = sf_stream_is_capturing(stream, &capturing);
+  if (st != SF_OK) return st;
+  if (!capturing)
     *bytes = static_cast<size_t>(M) * static_cast<size_t>(gathered_ld(K)) * 2;
   return SF_OK;
 }

@@ -422,6 +422,20 @@ int32_t sf_graph_destroy(void* exec) {
   return SF_OK;
 }
 
+int32_t sf_stream_is_capturing(void* stream, int32_t* capturing) {
+  if (!capturing) return fail(SF_ERR_INVALID_ARGUMENT, "null output");
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &st);
+  if (e == cudaErrorStreamCaptureImplicit) {
+    cudaGetLastError();
+    *capturing = 1;
+    return SF_OK;
+  }
+  SF_CUDA_TRY(e);
+  *capturing = st != cudaStreamCaptureStatusNone ? 1 : 0;
+  return SF_OK;
+}
+
 int32_t sf_can_access_peer(int32_t device, int32_t peer, int32_t* can) {
   if (!can) return fail(SF_ERR_INVALID_ARGUMENT, "null output");
   int c = 0;

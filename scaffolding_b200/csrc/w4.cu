@@ -423,7 +423,7 @@ int32_t run_w4(const W4Args& a, cudaStream_t s) {
       ceil_div(a.N, 128) * ceil_div(a.K, 128) >= kStreamBlocks)
     return a.M <= 8 ? launch_w4_stream_group<BF16, 1>(a, *dev, device, s)
                     : launch_w4_stream_group<BF16, 2>(a, *dev, device, s);
-  if (described && a.M > 16 && a.K > 0) {
+  if (described && a.M > 16) {
     if (a.group == 32) return launch_w4_tc<W4TcCfg<BF16, 1>>(a, *dev, device, s);
     if (a.group == 64) return launch_w4_tc<W4TcCfg<BF16, 2>>(a, *dev, device, s);
     return launch_w4_tc<W4TcCfg<BF16, 4>>(a, *dev, device, s);
@@ -550,7 +550,8 @@ int32_t sf_linear_w4(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx
     return fail(SF_ERR_INVALID_ARGUMENT, "unknown activation %d", activation);
   if (bias && !known_dtype(bias_dtype)) return fail(SF_ERR_INVALID_ARGUMENT, "unknown bias dtype");
   if (M == 0 || N == 0) return SF_OK;
-  if (!y || (K > 0 && !x)) return fail(SF_ERR_INVALID_ARGUMENT, "null pointer");
+  if (K == 0) return fail(SF_ERR_INVALID_ARGUMENT, "a 4-bit linear over no columns");
+  if (!y || !x) return fail(SF_ERR_INVALID_ARGUMENT, "null pointer");
   if (ldx < K || ldy < N) return fail(SF_ERR_INVALID_ARGUMENT, "leading dimension too small");
   const W4Args a{static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), x, ldx, packed, ldp,
                  scales, zeros, lds, group, in_dtype, bias, bias_dtype, y, ldy, out_dtype, activation,

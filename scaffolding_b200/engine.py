@@ -174,6 +174,13 @@ class PinnedHostBuffer:
             pass
 
 
+def stream_capturing(stream: int | None) -> bool:
+    """Whether work on ``stream`` is being captured into a graph."""
+    c = C.c_int32()
+    check(lib.sf_stream_is_capturing(stream, C.byref(c)), "sf_stream_is_capturing")
+    return bool(c.value)
+
+
 def memcpy(dst: int, src: int, nbytes: int, kind: int, stream: int | None = None) -> None:
     check(lib.sf_memcpy(C.c_void_p(dst), C.c_void_p(src), int(nbytes), kind,
                         C.c_void_p(stream) if stream else None), "sf_memcpy")

@@ -61,7 +61,7 @@ def check_route(ops, r, z, k, renormalize):
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("T,X,k", [(1, 8, 2), (1, 1, 1), (7, 3, 3), (64, 64, 4), (255, 31, 5),
-                                   (256, 128, 8), (257, 33, 1), (1000, 256, 8), (300, 1000, 32),
+                                   (256, 128, 8), (257, 33, 1), (1000, 256, 8), (300, 1000, 32), (256, 1024, 32), (200, 300, 16),
                                    (17776, 60, 2), (40000, 16, 4)])
 def test_route(gpu, ops, dt, T, X, k):
     rng = np.random.default_rng(T + X)
@@ -392,6 +392,64 @@ def test_moe_layer(gpu, ops, dt, act, T):
     tol = (4 * u + (hidden + dim) * 2.0 ** -22 + 2.0 ** -13 * (dt == "f32") + 2.0 ** -14) * mag
     tol += u * np.abs(ref) + TINY[dt]
     assert_within(y[clear], ref[clear], tol[clear], f"{dt} {act} {T}")
+    assert device_error(0) == 0
+
+
+def test_moe_layer_no_tokens_and_one_expert(gpu, ops):
+    from scaffolding_b200 import nn
+    rng = np.random.default_rng(0)
+    m = nn.MoE(32, 48, 1, 1, "silu", device=0, dtype=np_dtype("bf16"), rng=rng)
+    empty = ops._alloc((0, 32), np_dtype("bf16"), 0)
+    assert m(empty).shape == (0, 32)
+    gx, x = to_device(ops, rng.standard_normal((5, 32), dtype=np.float32), "bf16")
+    up = ops.dev_linear_forward(gx, ops.dev_reshape(m.up, (48, 32)), activation="silu")
+    ref = ops.dev_linear_forward(up, ops.dev_reshape(m.down, (32, 48)))
+    y, r = to_host32(ops, m(gx)), to_host32(ops, ref)  # one expert: weight 1
+    # the two products may round h, and then the sum, to neighbouring values
+    assert (np.abs(y - r) <= 4 * U["bf16"] * (np.abs(r) + np.abs(to_host32(ops, up)).sum(1, keepdims=True) / 7)).all()
+
+
+def test_decoder_feed_forward(gpu, ops):
+    """The operators as a sparse layer runs them in decoding: a 4-bit
+    projection, the routed experts with a residual, a 4-bit projection back,
+    each stage against 64 bits on the stage's own input; the same through
+    DataParallel on two shares of the one device."""
+    from scaffolding_b200 import nn
+    from scaffolding_b200.parallel import DataParallel
+    rng = np.random.default_rng(8)
+    dim, T = 256, 12
+    bf = np_dtype("bf16")
+    a = nn.Linear4.from_linear(nn.Linear(384, dim, device=0, rng=rng), 64, True, bf)
+    moe = nn.MoE(dim, 128, 8, 2, device=0, dtype=bf, rng=rng)
+    b = nn.Linear4.from_linear(nn.Linear(dim, 200, device=0, rng=rng), 128, False, bf)
+    gx, x = to_device(ops, rng.standard_normal((T, 384), dtype=np.float32), "bf16")
+
+    def linear4(m, v):
+        w = to_host32(ops, ops.dev_dequantize_w4(m.weight, np.float32)).astype(np.float64)
+        v = v.astype(np.float64)
+        ref = v @ w.T + to_host32(ops, m.bias)
+        # K + 2 K / group operations on terms of at most 15 |x| scale
+        s = np.repeat(to_host32(ops, m.weight.scales).astype(np.float64).T, m.weight.group, 1)[:, :w.shape[1]]
+        off = (w.shape[1] + 32) * 2.0 ** -23 * 15 * (np.abs(v) @ s.T) + 2.0 ** -24 * np.abs(ref)
+        return ref, off + U["bf16"] * (np.abs(ref) + off)
+
+    h = a(gx)
+    ref, tol = linear4(a, x)
+    assert_within(to_host32(ops, h).astype(np.float64), ref, tol)
+    e = moe(h, h)
+    hh = to_host32(ops, h)
+    ref, mag, gap = plain_moe(hh, [to_host32(ops, w) for w in (moe.router, moe.up, moe.down)], 2, "silu_gate",
+                              True, "bf16", hh)
+    clear = gap[:, 1] - gap[:, 2] > 2.0 ** -14
+    tol = (4 * U["bf16"] + 384 * 2.0 ** -22 + 2.0 ** -14) * mag + U["bf16"] * np.abs(ref)
+    assert_within(to_host32(ops, e).astype(np.float64)[clear], ref[clear], tol[clear])
+    y = b(e)
+    ref, tol = linear4(b, to_host32(ops, e))
+    assert_within(to_host32(ops, y).astype(np.float64), ref, tol)
+    whole = to_host32(ops, nn.Sequential(a, moe, b)(gx))
+    shares = to_host32(ops, DataParallel(nn.Sequential(a, moe, b), device_ids=[0, 0])(gx))
+    assert whole.shape == shares.shape == (T, 200)
+    assert np.abs(whole - shares).max() <= 2.0 ** -5 * np.abs(whole).max()
     assert device_error(0) == 0
 
 

@@ -121,6 +121,19 @@ def test_w4_refuses(ops):
         ops.dev_quantize_w4(_fake(ops, (4, 8), F16), group=16)
 
 
+def test_result_buffers_apart(ops):
+    """The result's buffer is not an input's (combine: not the rows')."""
+    x, w, off = _fake(ops, (10, 16)), _fake(ops, (3, 16, 16)), _fake(ops, (4,), I32)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.dev_grouped_linear(x, w, off, out=x)
+    y = _fake(ops, (4, 5))
+    with pytest.raises(ValueError, match="share memory"):
+        ops.dev_moe_combine(y, _fake(ops, (4, 1), I32), _fake(ops, (4, 1)), out=y)
+    h = _fake(ops, (6, 200), F16)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.dev_linear_w4(h, _w4(ops, N=200, dt=F16, K=200), out=h)
+
+
 def test_c_abi_refuses():
     from scaffolding_b200._lib import (SF_ERR_INVALID_ARGUMENT as BAD, SF_ERR_UNSUPPORTED as NO,
                                        SF_ERR_WORKSPACE, lib)
@@ -135,14 +148,16 @@ def test_c_abi_refuses():
     assert lib.sf_moe_route(10, 8, 2, None, 0, 8, 1, p, p, p, p, p, None, 0, None) == BAD
     assert lib.sf_moe_route(-1, 8, 2, p, 0, 8, 1, p, p, p, p, p, None, 0, None) == BAD
 
-    def grouped(groups=2, M=4, N=8, K=8, a_rows=4, lda=8, rows=None, off=p, ldb=8, ldc=8, dt=2, act=0, A=p):
-        return lib.sf_gemm_grouped(groups, M, N, K, A, a_rows, lda, rows, off, p, ldb, 64, None, 0, 0, p,
+    def grouped(groups=2, M=4, N=8, K=8, a_rows=4, lda=8, rows=None, off=p, ldb=8, ldc=8, dt=2, act=0, A=p,
+                b_stride=64):
+        return lib.sf_gemm_grouped(groups, M, N, K, A, a_rows, lda, rows, off, p, ldb, b_stride, None, 0, 0, p,
                                    ldc, dt, dt, act, None, 0, None)
 
     assert grouped(M=-1) == BAD and grouped(act=4) == BAD and grouped(dt=3) == BAD
     assert grouped(off=None) == BAD and grouped(A=None) == BAD
     assert grouped(a_rows=3) == BAD and grouped(lda=7) == BAD and grouped(ldb=7) == BAD and grouped(ldc=7) == BAD
     assert grouped(groups=5000) == NO and grouped(M=1 << 31, a_rows=1 << 31) == NO
+    assert grouped(M=(1 << 31) - 1, a_rows=(1 << 31) - 1) == NO and grouped(b_stride=-8) == BAD
     assert grouped(M=0) == 0 and grouped(groups=0) == 0 and grouped(N=0, ldc=0) == 0
 
     assert lib.sf_moe_combine(4, 8, 0, p, 8, 8, 2, p, p, None, 8, p, 8, None) == BAD
@@ -156,7 +171,7 @@ def test_c_abi_refuses():
 
     assert w4(M=65) == NO and w4(group=16) == NO and w4(in_dt=0) == NO
     assert w4(M=-1) == BAD and w4(packed=odd) == BAD and w4(ldp=18) == BAD and w4(ldp=12) == BAD
-    assert w4(lds=7) == BAD and w4(ldx=127) == BAD and w4(ldy=7) == BAD and w4(act=3) == BAD
+    assert w4(K=0, ldx=0) == BAD and w4(lds=7) == BAD and w4(ldx=127) == BAD and w4(ldy=7) == BAD and w4(act=3) == BAD
     assert w4(scales=None) == BAD and w4(M=0) == 0
     assert lib.sf_quantize_w4(8, 128, None, 0, 128, 128, p, 16, p, None, 8, 2, None) == BAD
     assert lib.sf_dequantize_w4(8, 128, p, 16, p, None, 8, 128, 2, p, 2, 127, None) == BAD

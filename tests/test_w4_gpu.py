@@ -144,6 +144,39 @@ def test_many_rows_dequantise(gpu, ops):
     assert np.array_equal(to_host32(ops, y), to_host32(ops, z))
 
 
+def test_many_rows_captured(gpu, ops):
+    """In a capture more than 64 rows run 64 at a time, with no memory of the
+    call's own in the graph; the replay gives the same bits as those calls."""
+    import ctypes as C
+
+    from scaffolding_b200 import engine as E
+    from scaffolding_b200._lib import check, lib
+    rng = np.random.default_rng(17)
+    w4, w, _ = weight(ops, rng, 100, 256, 64, "bf16", True)
+    gx, x = to_device(ops, rng.standard_normal((150, 256), dtype=np.float32), "bf16")
+    out = ops._alloc((150, 100), np_dtype("bf16"), 0)
+    parts = []
+    for m0 in (0, 64, 128):
+        px, _ = to_device(ops, x[m0:m0 + 64], "bf16")
+        parts.append(to_host32(ops, ops.dev_linear_w4(px, w4, activation="silu")))
+    s = ops.CudaStream(0)
+    E.set_stream(0, s.cuda_stream)
+    try:
+        check(lib.sf_graph_begin(C.c_void_p(s.cuda_stream)), "begin")
+        assert E.stream_capturing(s.cuda_stream)
+        ops.dev_linear_w4(gx, w4, activation="silu", out=out)
+        exe = C.c_void_p()
+        check(lib.sf_graph_end(C.c_void_p(s.cuda_stream), C.byref(exe)), "end")
+    finally:
+        E.set_stream(0, None)
+    assert not E.stream_capturing(s.cuda_stream) and not E.stream_capturing(None)
+    for _ in range(2):
+        check(lib.sf_graph_launch(exe, C.c_void_p(s.cuda_stream)), "launch")
+    s.synchronize()
+    assert np.array_equal(to_host32(ops, out), np.concatenate(parts))
+    check(lib.sf_graph_destroy(exe), "destroy")
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("group", [32, 128])
 @pytest.mark.parametrize("N,K", [(1, 1), (5, 200), (64, 384)])
