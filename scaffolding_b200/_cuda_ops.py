@@ -542,7 +542,7 @@ def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTen
     bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
     with E.on_device(dev):
         ws, ws_bytes = None, 0
-        if rows is not None:
+        if rows is not None and M > 1024:  # short batches need none
             need = C.c_size_t()
             check(lib.sf_gemm_grouped_workspace_size(X, M, N, K, E.dtype_code(gt_x.dtype),
                                                      E.get_stream(dev), C.byref(need)),

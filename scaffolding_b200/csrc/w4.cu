@@ -97,7 +97,7 @@ __device__ __forceinline__ void copy_async_wait() {
 
 // GW: 32-column words per group (1, 2, 4).
 template <bool BF16, int NT, int GW, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) w4_mma_kernel(const W4Args a, int wk, int x_vec) {
+__global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1) w4_mma_kernel(const W4Args a, int wk, int x_vec) {
   constexpr int NG = 4 / GW;             // groups per block
   constexpr int NA = w4_accumulators(NT, GW);
   constexpr int kSlot = (4 + 4 * NT) * 32;  // 16-byte vectors per block: a lane's words and x
@@ -176,13 +176,10 @@ __global__ void __launch_bounds__(32 * WARPS) w4_mma_kernel(const W4Args a, int 
     for (int u = 0; u < kW4Stages; ++u) {
       if (i0 + u >= mine) break;
       copy_block((u + kW4Stages - 1) % kW4Stages);
-      float sv[NG];
-      uint2 zv[NG];
+      uint32_t sv[NG];
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        sv[j] = (kw + (i0 + u) * wk) * NG + j < groups ? w4_float<BF16>(sc[u][j]) : 0.0f;
-        if (zeros) zv[j] = zero_pair<BF16>(ze[u][j]);
-      }
+      for (int j = 0; j < NG; ++j)
+        sv[j] = pack_scale<BF16>((kw + (i0 + u) * wk) * NG + j < groups ? sc[u][j] : 0u, ze[u][j], zeros);
       load_scales((u + 2) % 3);
       copy_async_wait<kW4Stages - 1>();
       uint4 q[4];
@@ -193,14 +190,7 @@ __global__ void __launch_bounds__(32 * WARPS) w4_mma_kernel(const W4Args a, int 
         float s[4];
         uint2 z[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[r] = __shfl_sync(0xffffffffu, sv[j], 8 * r + g);
-          z[r] = make_uint2(BF16 ? 0x43084308u : 0x64086408u, 0x54805480u);  // + 8
-          if (zeros) {
-            z[r].x = __shfl_sync(0xffffffffu, zv[j].x, 8 * r + g);
-            if constexpr (!BF16) z[r].y = __shfl_sync(0xffffffffu, zv[j].y, 8 * r + g);
-          }
-        }
+        for (int r = 0; r < 4; ++r) unpack_scale<BF16>(__shfl_sync(0xffffffffu, sv[j], 8 * r + g), s[r], z[r]);
         float sum[2][NT][NA][4] = {};
 #pragma unroll
         for (int l = 0; l < GW; ++l) {

@@ -155,22 +155,14 @@ __global__ void __launch_bounds__(Cfg::THREADS, 4)
           q[r] = *reinterpret_cast<const uint4*>(words + u * Cfg::STAGE_BYTES + r * 512);
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          const float sv = w4_float<BF16>(*reinterpret_cast<const uint16_t*>(ss + u * Cfg::STAGE_BYTES + j * 256));
-          uint2 zv;
-          if (zeros)
-            zv = zero_pair<BF16>(
-                *reinterpret_cast<const uint16_t*>(ss + u * Cfg::STAGE_BYTES + Cfg::S_BYTES + j * 256));
+          const uint8_t* at = ss + u * Cfg::STAGE_BYTES + j * 256;
+          const uint32_t sv = pack_scale<BF16>(
+              *reinterpret_cast<const uint16_t*>(at),
+              zeros ? *reinterpret_cast<const uint16_t*>(at + Cfg::S_BYTES) : 0u, zeros);
           float s[4];
           uint2 z[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            s[r] = __shfl_sync(0xffffffffu, sv, 8 * r + g);
-            z[r] = make_uint2(BF16 ? 0x43084308u : 0x64086408u, 0x54805480u);  // + 8
-            if (zeros) {
-              z[r].x = __shfl_sync(0xffffffffu, zv.x, 8 * r + g);
-              if constexpr (!BF16) z[r].y = __shfl_sync(0xffffffffu, zv.y, 8 * r + g);
-            }
-          }
+          for (int r = 0; r < 4; ++r) unpack_scale<BF16>(__shfl_sync(0xffffffffu, sv, 8 * r + g), s[r], z[r]);
           float sum[2][NT][NA][4] = {};
 #pragma unroll
           for (int l = 0; l < GW; ++l) {

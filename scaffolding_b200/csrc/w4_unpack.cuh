@@ -109,6 +109,25 @@ __device__ __forceinline__ uint2 zero_pair(uint32_t v) {
   return r;
 }
 
+// A row's scale and the pair constant of its zero, as one word for a shuffle:
+// the scale's bits below, the first constant's above.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_scale(uint32_t scale, uint32_t zero, bool zeros) {
+  const uint32_t z = zeros ? zero_pair<BF16>(zero).x : (BF16 ? 0x43084308u : 0x64086408u);  // + 8
+  return __byte_perm(scale, z, 0x5410);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void unpack_scale(uint32_t v, float& s, uint2& z) {
+  s = w4_float<BF16>(v & 0xFFFFu);
+  z.x = __byte_perm(v, v, 0x3232);
+  z.y = 0;
+  if constexpr (!BF16) {
+    const __half2 n = __hsub2(*reinterpret_cast<const __half2*>(&z.x), __float2half2_rn(960.0f));
+    z.y = *reinterpret_cast<const uint32_t*>(&n);
+  }
+}
+
 // Accumulators of one 16 x 8 tile and group.  An mma.sync that adds to the result
 // of the one before it waits about 140 cycles for it (a block of eight chained
 // ones took 1100 cycles, in two chains of four 534), so a group's mmas go round
