@@ -220,7 +220,8 @@ int32_t sf_moe_combine(int64_t tokens, int64_t cols, int32_t top_k, const void* 
 /* y[M,N] = act(x[M,K] . W[N,K]^T + bias) with
  *   W[n, k] = scales[k / group, n] * (q[n, k] - zeros[k / group, n]),
  * q in 0..15, zeros = 8 when NULL, for M <= 64 rows of bf16/fp16 x (the
- * weights are read once per 16 rows).  scales and zeros are
+ * weights are read once; once per 16 rows where x starts off 16 bytes).
+ * scales and zeros are
  * [ceil(K / group)][lds >= N] in x's type; a zero stands for the whole number
  * in 0..15 nearest to it; group is 32, 64 or 128.  packed row n holds ldp >= 16 *
  * ceil(K / 128) words (16-byte aligned, ldp a multiple of 4): nibble i (from

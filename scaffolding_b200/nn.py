@@ -145,8 +145,7 @@ class MoE:
 
     router ``[experts, dim]``, ``up`` ``[experts, hidden, dim]`` (``[experts,
     2 hidden, dim]`` for ``silu_gate``), ``down`` ``[experts, dim, hidden]``,
-    all drawn like Linear's weights.  Five launches for a decoding batch, six
-    for a prompt; the group sizes never leave the device."""
+    all drawn like Linear's weights.  The group sizes never leave the device."""
 
     def __init__(self, dim: int, hidden: int, num_experts: int, top_k: int = 2,
                  activation: str = "silu_gate", renormalize: bool = True, device=None,

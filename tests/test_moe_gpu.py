@@ -33,7 +33,7 @@ def plain_route(z, k, renormalize):
         over = picked[t] if renormalize else z[t]
         if top == -np.inf:
             continue
-        e = lambda v: np.where(v == top, 1.0, np.exp(np.where(v == top, 0.0, v - top)))  # noqa: E731
+        e = lambda v: np.exp(np.subtract(v, top, out=np.zeros_like(v), where=v != top))  # noqa: E731
         weights[t] = e(picked[t]) / e(over).sum()
     flat = experts.reshape(-1)
     order = np.argsort(flat, kind="stable")
