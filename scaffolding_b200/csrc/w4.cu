@@ -309,20 +309,60 @@ int32_t encode_words(CUtensorMap* m, const W4Args& a, CUtensorMapSwizzle swizzle
   return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.packed, 2, dims, strides, box, swizzle);
 }
 
+// CTAs per 128 rows of the streaming kernel: the largest cluster with which all
+// clusters run at once, since a second wave costs as much as the first.  The
+// launch before this one leaves its places one by one, so a sixteenth is kept
+// free.  8192 -> 11008, one row: 38.6 / 32.3 / 23.8 / 19.4 / 17.0 / 15.4 us in
+// clusters of 1 to 6, 19.9 in 8 (two waves); 5120 -> 14336: 14.2 in 4, 16.8 in 5,
+// which fill the device to the last place.  Where nothing fits, the fewest that
+// are more than two per SM (8192 -> 28672, one row: 62.6 / 34.9 / 37.4 / 35.9 us
+// for 1 / 2 / 3 / 4).  This is those fewest; 9 if 8 are not enough.
+int least_stream_splits(int64_t tiles, int sm_count) {
+  int s = 1;
+  while (s <= 8 && tiles * s <= 2 * sm_count) ++s;
+  return s;
+}
+
 // Blocks of 128 x 128 from which the streaming kernel is used.  Its clusters and
 // its CTA-wide pipeline cost about 3 us more to start and to end than the ring
-// kernel's, and it streams faster.  Ring / stream, one row of x, group 128: 5.1 /
-// 6.9 us at 4096 x 4096 (1024 blocks), 10.3 / 10.0 us at 4096 -> 11008 (2752),
-// 38.9 / 34.1 us at 8192 -> 28672 (14336); 16 rows there: 76 / 59 us.
-constexpr int64_t kStreamBlocks = 4096;
+// kernel's, and it streams faster, with 9 to 16 rows by more.  Ring / stream,
+// groups of 128, one row of x: 6.7 / 8.0 us at 4096 -> 8192 (2048 blocks), 9.8 /
+// 10.2 us at 4096 -> 11008 (2752), 16.7 / 15.2 us at 4096 -> 22016 (5504), 38.6 /
+// 34.6 us at 8192 -> 28672 (14336); 16 rows: 6.7 / 10.2 us at 4096 x 4096 (1024),
+// 13.0 / 11.6, 18.7 / 15.3, 31.2 / 23.0, 68.9 / 51.0 us.  And it needs its CTAs: one
+// row 13.0 / 19.0 us at 16384 -> 4096, where clusters of 8 are 256 of them.
+constexpr int64_t kStreamBlocks = 4096, kStreamBlocks16 = 2048;
 
-// CTAs per 128 rows of the streaming kernel: as many as give every SM three
-// (8192 -> 28672: 62 / 34 / 38 / 36 / 36 / 39 us for 1 / 2 / 3 / 4 / 5 / 8).
-int pick_stream_splits(const W4Args& a, int sm_count) {
-  const int64_t tiles = ceil_div(a.N, 128), blocks = ceil_div(a.K, 128);
-  int s = 1;
-  while (s < 8 && s * 4 <= blocks && tiles * s < 3 * sm_count) s *= 2;
-  return s;
+bool use_stream(const W4Args& a, int sm_count) {
+  const int64_t tiles = ceil_div(a.N, 128);
+  return least_stream_splits(tiles, sm_count) <= 8 &&
+         tiles * ceil_div(a.K, 128) >= (a.M <= 8 ? kStreamBlocks : kStreamBlocks16);
+}
+
+// Clusters of 1 to 8 CTAs of a kernel that fit the device at once: how many CTAs
+// an SM holds, and what packing whole clusters into its groups of SMs leaves over.
+// Asked once per kernel and device.
+template <class Kernel>
+int32_t cluster_capacity(Kernel kernel, int threads, int smem, int device, std::atomic<int> (&known)[64][8],
+                         int splits, int* out) {
+  std::atomic<int>& entry = known[device][splits - 1];
+  int n = entry.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(splits));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SF_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    entry.store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return SF_OK;
 }
 
 template <class Cfg>
@@ -348,7 +388,18 @@ int32_t launch_w4_stream(const W4Args& a, const DeviceInfo& dev, int device, cud
   static std::atomic<bool> allowed[64];
   st = allow_smem(w4_stream_kernel<Cfg>, Cfg::SMEM_BYTES, device, allowed);
   if (st != SF_OK) return st;
-  const int splits = pick_stream_splits(a, dev.sm_count);
+  static std::atomic<int> known[64][8];
+  const int64_t tiles = ceil_div(a.N, 128);
+  int splits = least_stream_splits(tiles, dev.sm_count);
+  for (int c = 8; c > splits; --c) {
+    int fit = 0;
+    st = cluster_capacity(w4_stream_kernel<Cfg>, Cfg::THREADS, Cfg::SMEM_BYTES, device, known, c, &fit);
+    if (st != SF_OK) return st;
+    if (tiles * 16 <= static_cast<int64_t>(fit) * 15) {
+      splits = c;
+      break;
+    }
+  }
   return launch_cluster(w4_stream_kernel<Cfg>, ceil_div(a.N, 128) * splits, Cfg::THREADS, Cfg::SMEM_BYTES, splits, s,
                         mw, mx, ms, mz, a, splits, dev.err_word);
 }
@@ -410,7 +461,7 @@ int32_t run_w4(const W4Args& a, cudaStream_t s) {
   int32_t st = current_device_info(&dev, &device);
   if (st != SF_OK) return st;
   if (described && a.M <= 16 && a.K % 32 == 0 && a.lds % 8 == 0 && aligned16(a.scales) && aligned16(a.zeros) &&
-      ceil_div(a.N, 128) * ceil_div(a.K, 128) >= kStreamBlocks)
+      use_stream(a, dev->sm_count))
     return a.M <= 8 ? launch_w4_stream_group<BF16, 1>(a, *dev, device, s)
                     : launch_w4_stream_group<BF16, 2>(a, *dev, device, s);
   if (described && a.M > 16) {

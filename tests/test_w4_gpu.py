@@ -101,9 +101,20 @@ def test_linear_wide(gpu, ops, dt):
 @pytest.mark.parametrize("M", [1, 5, 16])
 def test_linear_streamed(gpu, ops, dt, group, zeros, M):
     """Sizes of the streaming kernel (4096 blocks of 128 x 128 and more, up to
-    16 rows): a last tile of 8 rows, a last block cut short, clusters of two."""
+    16 rows): a last tile of 8 rows, a last block cut short, clusters of four."""
     rng = np.random.default_rng(M)
     run(ops, rng, dt, M, 16392, 4064, group, zeros, "silu", True)
+    assert device_error(0) == 0
+
+
+@pytest.mark.parametrize("N,K", [(5000, 6880), (8900, 3840), (11008, 3104), (12700, 2720), (16392, 2080),
+                                 (22000, 1568), (37888, 1024), (41000, 864)])
+def test_linear_streamed_clusters(gpu, ops, N, K):
+    """Rows and columns whose clusters are of each size from eight down to one;
+    nine rows of x, whose sums the CTAs share out unevenly."""
+    rng = np.random.default_rng(N)
+    run(ops, rng, "bf16", 9, N, K, 128, True)
+    run(ops, rng, "f16", 16, N, K, 32, False, "silu", True)
     assert device_error(0) == 0
 
 
