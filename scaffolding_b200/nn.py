@@ -179,11 +179,13 @@ class MoE:
     def forward(self, x: GpuTensor, residual: GpuTensor | None = None) -> GpuTensor:
         """``x [..., dim]`` to the same shape; ``residual`` (that shape too)
         is added to the experts' sum before it is rounded."""
+        if x.ndim < 1 or x.shape[-1] != self.dim:
+            raise ValueError(f"MoE of width {self.dim}: x {x.shape}")
         if self.router.device_id != x.device_id:
             self.to(x.device_id)
         if residual is not None and residual.shape != x.shape:
             raise ValueError(f"residual must be {x.shape}, got {residual.shape}")
-        flat = ops.dev_reshape(x, (x.numel // self.dim, self.dim))
+        flat = ops.dev_reshape(x, (math.prod(x.shape[:-1]), self.dim))
         logits = ops.dev_linear_forward(flat, self.router, out_dtype=np.float32)
         route = ops.dev_moe_route(logits, self.top_k, self.renormalize)
         h = ops.dev_grouped_linear(flat, self.up, route.offsets, activation=self.activation,
