@@ -540,21 +540,26 @@ def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTen
     odt = _out_dtype(gt_x, out_dtype if out is None else out.dtype)
     y = _result(out, (M, N), odt, dev, "out")
     bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
-    with E.on_device(dev):
-        ws, ws_bytes = None, 0
-        if rows is not None and M > 1024:  # short batches need none
-            need = C.c_size_t()
-            check(lib.sf_gemm_grouped_workspace_size(X, M, N, K, E.dtype_code(gt_x.dtype),
-                                                     E.get_stream(dev), C.byref(need)),
-                  "sf_gemm_grouped_workspace_size")
-            if need.value:
-                buf = E.workspace(dev, E.get_stream(dev), need.value)
-                ws, ws_bytes = buf.ptr, buf.nbytes
+    stream, code = E.get_stream(dev), E.dtype_code(gt_x.dtype)
+
+    def launch(ws, ws_bytes):
         check(lib.sf_gemm_grouped(X, M, N, K, _ptr(gt_x), gt_x.shape[0], K, _ptr(rows),
                                   _ptr(gt_offsets), _ptr(gt_weight), K, wide * K, _ptr(gt_bias),
-                                  bias_dt, wide, _ptr(y), N, E.dtype_code(gt_x.dtype),
-                                  E.dtype_code(odt), act, ws, ws_bytes, E.get_stream(dev)),
+                                  bias_dt, wide, _ptr(y), N, code, E.dtype_code(odt), act, ws,
+                                  ws_bytes, stream),
               "sf_gemm_grouped")
+
+    with E.on_device(dev):
+        need = C.c_size_t()
+        if rows is not None and M > 1024:  # short batches need none
+            check(lib.sf_gemm_grouped_workspace_size(X, M, N, K, code, stream, C.byref(need)),
+                  "sf_gemm_grouped_workspace_size")
+        if need.value:
+            with E.workspace_lock:
+                buf = E.workspace(dev, stream, need.value)
+                launch(buf.ptr, buf.nbytes)
+        else:
+            launch(None, 0)
     return y
 
 

@@ -193,17 +193,22 @@ def stream_sync(stream: int | None) -> None:
 
 # ───────────────────────────── workspaces ─────────────────────────────
 
-_ws_lock = threading.Lock()
+# Held from the lookup of a workspace until the last launch that uses it is
+# queued.  Launches on one stream run in order, so a queued call is safe from
+# the next one; but a call may be several launches (a gather and its product, a
+# split-K sum and its finaliser), between which another host thread's must not
+# come, and a buffer that is outgrown is freed.
+workspace_lock = threading.RLock()
 _workspaces: dict[tuple[int, int], DeviceBuffer] = {}
 
 
 def workspace(dev: int, stream: int | None, nbytes: int) -> DeviceBuffer | None:
-    """Per-(device, stream) scratch buffer, grown on demand.  Launches on one
-    stream are ordered, so reusing it across calls on that stream is safe."""
+    """Per-(device, stream) scratch buffer, grown on demand; called, and its
+    launches queued, with ``workspace_lock`` held."""
     if nbytes <= 0:
         return None
     key = (dev, int(stream or 0))
-    with _ws_lock:
+    with workspace_lock:
         buf = _workspaces.get(key)
         if buf is None or buf.nbytes < nbytes:
             if buf is not None:
@@ -215,7 +220,7 @@ def workspace(dev: int, stream: int | None, nbytes: int) -> DeviceBuffer | None:
 
 
 def release_workspaces() -> None:
-    with _ws_lock:
+    with workspace_lock:
         for b in _workspaces.values():
             b.free()
         _workspaces.clear()
@@ -259,20 +264,26 @@ def gemm(M, N, K, A, lda, trans_a, B, ldb, trans_b, Cp, ldc, in_dt, out_dt, *,
     check(lib.sf_gemm_workspace_size(C.byref(batch) if batch is not None else None,
                                      M, N, K, trans_a, trans_b, in_dt, out_dt, C.byref(need)),
           "sf_gemm_workspace_size")
-    ws = workspace(dev, stream, need.value)
-    wsp = C.c_void_p(ws.ptr) if ws else None
-    wsb = ws.nbytes if ws else 0
-    ep = C.byref(epi) if epi is not None else None
-    sp = C.c_void_p(stream) if stream else None
-    if batch is None:
-        st = lib.sf_gemm(M, N, K, C.c_void_p(A), lda, trans_a, C.c_void_p(B), ldb, trans_b,
-                         C.c_void_p(Cp), ldc, in_dt, out_dt, ep, wsp, wsb, sp)
-        check(st, "sf_gemm")
+    if need.value:
+        with workspace_lock:
+            ws = workspace(dev, stream, need.value)
+            _gemm_launch(M, N, K, A, lda, trans_a, B, ldb, trans_b, Cp, ldc, in_dt, out_dt, epi, batch,
+                         ws.ptr, ws.nbytes, stream)
     else:
-        st = lib.sf_gemm_batched(C.byref(batch), M, N, K, C.c_void_p(A), lda, trans_a,
-                                 C.c_void_p(B), ldb, trans_b, C.c_void_p(Cp), ldc, in_dt, out_dt,
-                                 ep, wsp, wsb, sp)
-        check(st, "sf_gemm_batched")
+        _gemm_launch(M, N, K, A, lda, trans_a, B, ldb, trans_b, Cp, ldc, in_dt, out_dt, epi, batch,
+                     None, 0, stream)
+
+
+def _gemm_launch(M, N, K, A, lda, trans_a, B, ldb, trans_b, Cp, ldc, in_dt, out_dt, epi, batch,
+                 ws, ws_bytes, stream) -> None:
+    ep = C.byref(epi) if epi is not None else None
+    if batch is None:
+        check(lib.sf_gemm(M, N, K, A, lda, trans_a, B, ldb, trans_b, Cp, ldc, in_dt, out_dt, ep,
+                          ws, ws_bytes, stream or None), "sf_gemm")
+    else:
+        check(lib.sf_gemm_batched(C.byref(batch), M, N, K, A, lda, trans_a, B, ldb, trans_b, Cp,
+                                  ldc, in_dt, out_dt, ep, ws, ws_bytes, stream or None),
+              "sf_gemm_batched")
 
 
 def softmax_rows(x, x_dt, ldx, y, y_dt, ldy, rows, cols, scale=1.0, stream=None, device=None):

@@ -1,0 +1,56 @@
+"""Calls of the routed and the 4-bit linears that a program makes and a single
+call in a quiet process does not show (-m gpu): several host threads, captured
+modules, uploads beside queued work, the sizes at which the kernels' rings,
+clusters and accumulators come round."""
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+from tests.gpu_util import device_error, np_dtype, to_device, to_host32
+
+pytestmark = pytest.mark.gpu
+
+
+def _in_threads(*calls):
+    """Every call in a thread of its own, started together."""
+    errors, gate = [], threading.Barrier(len(calls))
+
+    def run(fn):
+        try:
+            gate.wait(30)
+            fn()
+        except BaseException as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(fn,)) for fn in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not errors and not any(t.is_alive() for t in threads), errors
+
+
+def test_gathered_batches_of_two_threads(gpu, ops):
+    """Two threads on the default stream, each with gathered batches of its own
+    that go through the stream's workspace, the second's larger at times: the
+    bits of the same calls made one by one."""
+    rng = np.random.default_rng(5)
+    X, K, N, T = 4, 64, 1024, 300
+    gw, _ = to_device(ops, rng.standard_normal((X, N, K), dtype=np.float32), "bf16")
+    jobs = []
+    for M in (2100, 2400, 4300):
+        gx, _ = to_device(ops, rng.standard_normal((T, K), dtype=np.float32), "bf16")
+        rows = ops.gputensor_from_numpy(rng.integers(0, T, M).astype(np.int32))
+        off = ops.gputensor_from_numpy(np.array([0, M // 3, M // 2, M - 7, M], np.int32))
+        want = to_host32(ops, ops.dev_grouped_linear(gx, gw, off, rows=rows))
+        jobs.append((gx, off, rows, want))
+
+    def loop(which):
+        for i in range(40):
+            gx, off, rows, want = jobs[which[i % len(which)]]
+            assert np.array_equal(to_host32(ops, ops.dev_grouped_linear(gx, gw, off, rows=rows)), want)
+
+    _in_threads(lambda: loop([0]), lambda: loop([1, 2]))
+    assert device_error(0) == 0

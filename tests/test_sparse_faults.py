@@ -1,6 +1,8 @@
 """Faults of the routed and the 4-bit linears that the host alone decides:
 refused shapes, shared memory, the order of launches.  CPU only: the engine's
 entry points are stood in for where a call would reach a device."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -30,3 +32,136 @@ def test_moe_refuses_another_width(ops):
     for shape in ((4, 128), (2, 3, 640), (64, 1), (8, 32), (128,), ()):
         with pytest.raises(ValueError, match="width 64"):
             m(_fake(ops, shape))
+
+
+class _Engine:
+    """Stands in for the entry points behind the engine's launches and memory:
+    a log of (call, thread, what), and memory that is only addresses."""
+
+    def __init__(self, monkeypatch):
+        from scaffolding_b200._lib import lib
+        self.lib, self.log, self.mu = lib, [], threading.Lock()
+        self.next, self.freed, self.capture_id = 1 << 20, {}, {}
+        self.patch = lambda name, fn: monkeypatch.setattr(lib, name, fn)
+        self.patch("sf_malloc", self._malloc)
+        self.patch("sf_free", self._free)
+        self.patch("sf_get_device", lambda out: self._set(out, 0))
+        self.patch("sf_set_device", lambda dev: 0)
+        self.patch("sf_device_synchronize", lambda: self.note("device sync", None))
+        self.patch("sf_stream_synchronize", lambda s: self.note("sync", s))
+
+    @staticmethod
+    def _set(out, value):
+        out._obj.value = value
+        return 0
+
+    def note(self, call, what):
+        with self.mu:
+            self.log.append((call, threading.get_ident(), what))
+        return 0
+
+    def _malloc(self, dev, nbytes, out):
+        """The pool's rule: a freed block of the same size comes back first."""
+        with self.mu:
+            size = -(-max(nbytes, 1) // 256) * 256
+            if self.freed.get(size):
+                return self._set(out, self.freed[size].pop())
+            p, self.next = self.next, self.next + size
+        return self._set(out, p)
+
+    def _free(self, dev, p, nbytes):
+        size = -(-max(nbytes, 1) // 256) * 256
+        with self.mu:
+            self.freed.setdefault(size, []).append(p.value)
+            self.log.append(("free", threading.get_ident(), p.value))
+        return 0
+
+
+@pytest.fixture
+def engine(monkeypatch):
+    from scaffolding_b200 import engine as E
+    monkeypatch.setattr(E, "_workspaces", {})
+    monkeypatch.setattr(E, "_streams", {})
+    return _Engine(monkeypatch)
+
+
+def _grouped_needs(engine, nbytes):
+    engine.patch("sf_gemm_grouped_workspace_size", lambda X, M, N, K, dt, s, out: engine._set(out, nbytes(M)))
+
+
+def _two_threads(first, second, inside):
+    """Runs ``first`` until ``inside`` is set within it, then ``second`` beside it."""
+    errors = []
+
+    def guarded(fn):
+        try:
+            fn()
+        except BaseException as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    a = threading.Thread(target=guarded, args=(first,))
+    b = threading.Thread(target=guarded, args=(second,))
+    a.start()
+    assert inside.wait(10)
+    b.start()
+    a.join(20)
+    b.join(20)
+    assert not a.is_alive() and not b.is_alive() and not errors, errors
+
+
+@pytest.mark.parametrize("grow", [False, True])
+def test_gathered_rows_of_two_threads(ops, engine, grow):
+    """A gathered batch makes two launches through the stream's workspace: no
+    other thread's launch comes between them, and none frees it for a larger
+    one while the first has its address."""
+    inside, done = threading.Event(), threading.Event()
+
+    def launch(X, M, N, K, *rest):
+        ws = rest[16]
+        engine.note("enter", ws)
+        if not inside.is_set():
+            inside.set()
+            done.wait(0.5)  # room for the other thread to come between
+        engine.note("leave", ws)
+        done.set()
+        return 0
+
+    engine.patch("sf_gemm_grouped", launch)
+    _grouped_needs(engine, lambda M: M * 32)
+    w, off = _fake(ops, (3, 8, 16), F16), _fake(ops, (4,), I32)
+
+    def call(M):
+        ops.dev_grouped_linear(_fake(ops, (10, 16), F16), w, off, rows=_fake(ops, (M,), I32),
+                               out=ops.GpuTensor(ops.CudaBuffer(64, 16, 0, False), (M, 8), F16, 0))
+
+    _two_threads(lambda: call(3000), lambda: call(9000 if grow else 3000), inside)
+    seen = [(c, t) for c, t, _ in engine.log if c in ("enter", "leave", "free")]
+    first = seen[0][1]
+    end = seen.index(("leave", first))
+    assert seen[0][0] == "enter" and all(t == first for _, t in seen[:end]), seen
+
+
+def test_split_k_of_two_threads(ops, engine):
+    """The same rule for a GEMM whose split-K sums lie in the workspace."""
+    from scaffolding_b200 import engine as E
+    inside, done = threading.Event(), threading.Event()
+
+    def launch(*args):
+        engine.note("enter", None)
+        if not inside.is_set():
+            inside.set()
+            done.wait(0.5)
+        engine.note("leave", None)
+        done.set()
+        return 0
+
+    engine.patch("sf_gemm", launch)
+    engine.patch("sf_gemm_workspace_size", lambda *a: engine._set(a[-1], a[1] * 64))
+
+    def call(M):
+        E.gemm(M, 8, 8, 64, 8, 0, 64, 8, 1, 64, 8, 0, 0, device=0)
+
+    _two_threads(lambda: call(4), lambda: call(400), inside)
+    seen = [(c, t) for c, t, _ in engine.log if c in ("enter", "leave", "free")]
+    end = seen.index(("leave", seen[0][1]))
+    assert all(t == seen[0][1] for _, t in seen[:end]), seen
