@@ -220,7 +220,11 @@ def workspace(dev: int, stream: int | None, nbytes: int) -> DeviceBuffer | None:
 
 
 def release_workspaces() -> None:
+    """Return the workspaces to the pool once nothing queued uses them."""
     with workspace_lock:
+        for dev in {key[0] for key in _workspaces}:
+            with on_device(dev):
+                check(lib.sf_device_synchronize(), "sf_device_synchronize")
         for b in _workspaces.values():
             b.free()
         _workspaces.clear()

@@ -165,3 +165,14 @@ def test_split_k_of_two_threads(ops, engine):
     seen = [(c, t) for c, t, _ in engine.log if c in ("enter", "leave", "free")]
     end = seen.index(("leave", seen[0][1]))
     assert all(t == seen[0][1] for _, t in seen[:end]), seen
+
+
+def test_released_workspaces_are_not_in_use(engine):
+    """A workspace goes back to the pool only when no queued launch reads it."""
+    from scaffolding_b200 import engine as E
+    with E.workspace_lock:
+        ptr = E.workspace(0, 77, 4096).ptr
+    E.release_workspaces()
+    calls = [(c, what) for c, _, what in engine.log]
+    assert ("free", ptr) in calls and calls.index(("device sync", None)) < calls.index(("free", ptr))
+    assert not E._workspaces
