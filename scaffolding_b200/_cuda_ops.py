@@ -698,15 +698,19 @@ def dev_dequantize_w4(weight: W4Weight, dtype=None) -> GpuTensor:
     """The ``[N, K]`` weight a W4Weight stands for, in ``dtype`` (default: its
     scales' type), each value rounded once."""
     n, k = weight.shape
+    w = _alloc((n, k), np.dtype(dtype) if dtype is not None else weight.scales.dtype, weight.device_id)
+    _dequantize_into(weight, w)
+    return w
+
+
+def _dequantize_into(weight: W4Weight, w: GpuTensor) -> None:
+    n, k = weight.shape
     dev = weight.device_id
-    wdt = np.dtype(dtype) if dtype is not None else weight.scales.dtype
-    w = _alloc((n, k), wdt, dev)
     with E.on_device(dev):
         check(lib.sf_dequantize_w4(n, k, _ptr(weight.packed), weight.packed.shape[1],
                                    _ptr(weight.scales), _ptr(weight.zeros), n, weight.group,
-                                   E.dtype_code(weight.scales.dtype), _ptr(w), E.dtype_code(wdt), k,
+                                   E.dtype_code(weight.scales.dtype), _ptr(w), E.dtype_code(w.dtype), k,
                                    E.get_stream(dev)), "sf_dequantize_w4")
-    return w
 
 
 def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None = None,
@@ -714,11 +718,11 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
     """``dev_linear_forward`` over a 4-bit weight: ``act(x @ W^T + bias)`` for
     bf16 / fp16 x.  Up to 64 rows of x run on ``sf_linear_w4``, which streams
     the packed weight; more rows dequantise it into a 16-bit weight (one more
-    rounding per weight, which the streamed product does not make) and run
-    the GEMM.  During a graph capture more rows run 64 at a time on
-    ``sf_linear_w4`` instead: a graph must not hold the dequantised weight,
-    whose memory is free again when the call returns.  ``out`` shares no
-    memory with x."""
+    rounding per weight, which the streamed product does not make) in the
+    stream's workspace and run the GEMM.  During a graph capture more rows run
+    64 at a time on ``sf_linear_w4`` instead: a graph must not hold the
+    dequantised weight, whose memory the stream's next call uses again.
+    ``out`` shares no memory with x."""
     act = E.act_code(activation)
     if gt_x.dtype != weight.scales.dtype:
         raise TypeError(f"x and the weight's scales must share a dtype ({gt_x.dtype} vs {weight.scales.dtype})")
@@ -738,7 +742,7 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
     in_code, out_code = E.dtype_code(gt_x.dtype), E.dtype_code(odt)
     stream = E.get_stream(dev)
     with E.on_device(dev):
-        if M <= _W4_MAX_ROWS or E.stream_capturing(stream):
+        if M <= _W4_MAX_ROWS or n == 0 or E.stream_capturing(stream):
             x_row, y_row = k * gt_x.dtype.itemsize, n * odt.itemsize
             for m0 in range(0, M, _W4_MAX_ROWS):
                 check(lib.sf_linear_w4(min(M - m0, _W4_MAX_ROWS), n, k, gt_x.ptr + m0 * x_row, k,
@@ -747,11 +751,14 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
                                        _ptr(gt_bias), bias_dt, y.ptr + m0 * y_row, n, in_code,
                                        out_code, act, stream), "sf_linear_w4")
         else:
-            w = dev_dequantize_w4(weight)
             epi = E.make_epilogue(bias_ptr=gt_bias.ptr if gt_bias is not None else 0,
                                   bias_dt=bias_dt, act=act)
-            E.gemm(M, n, k, gt_x.ptr, k, 0, w.ptr, k, 1, y.ptr, n, in_code, out_code, epi=epi,
-                   device=dev)
+            with E.workspace_lock:
+                buf = E.workspace(dev, stream, n * k * gt_x.dtype.itemsize, "weight")
+                w = GpuTensor(buf, (n, k), gt_x.dtype, dev)
+                _dequantize_into(weight, w)
+                E.gemm(M, n, k, gt_x.ptr, k, 0, w.ptr, k, 1, y.ptr, n, in_code, out_code, epi=epi,
+                       device=dev)
     return y
 
 

@@ -199,15 +199,17 @@ def stream_sync(stream: int | None) -> None:
 # split-K sum and its finaliser), between which another host thread's must not
 # come, and a buffer that is outgrown is freed.
 workspace_lock = threading.RLock()
-_workspaces: dict[tuple[int, int], DeviceBuffer] = {}
+_workspaces: dict[tuple[int, int, str], DeviceBuffer] = {}
 
 
-def workspace(dev: int, stream: int | None, nbytes: int) -> DeviceBuffer | None:
-    """Per-(device, stream) scratch buffer, grown on demand; called, and its
-    launches queued, with ``workspace_lock`` held."""
+def workspace(dev: int, stream: int | None, nbytes: int, use: str = "sums") -> DeviceBuffer | None:
+    """Per-(device, stream, use) scratch buffer, grown on demand; called, and
+    its launches queued, with ``workspace_lock`` held.  What a call has in two
+    buffers at once are two uses.  It is memory that no allocation can take
+    while queued launches use it: the pool does not know of streams."""
     if nbytes <= 0:
         return None
-    key = (dev, int(stream or 0))
+    key = (dev, int(stream or 0), use)
     with workspace_lock:
         buf = _workspaces.get(key)
         if buf is None or buf.nbytes < nbytes:

@@ -54,3 +54,34 @@ def test_gathered_batches_of_two_threads(gpu, ops):
 
     _in_threads(lambda: loop([0]), lambda: loop([1, 2]))
     assert device_error(0) == 0
+
+
+@pytest.fixture
+def own_stream(gpu, ops):
+    """The engine's launches on a non-blocking stream, which the uploads of the
+    legacy stream do not wait for by themselves."""
+    from scaffolding_b200 import engine as E
+    s = ops.CudaStream(0)
+    E.set_stream(0, s.cuda_stream)
+    yield s
+    s.synchronize()
+    E.set_stream(0, None)
+
+
+def test_upload_beside_an_unpacked_weight(ops, own_stream):
+    """Uploads of tensors of the unpacked weight's size right after 4-bit
+    linears of many rows, whose products are still queued."""
+    rng = np.random.default_rng(9)
+    N, K, M = 1024, 2048, 4000
+    gw, _ = to_device(ops, rng.standard_normal((N, K), dtype=np.float32), "bf16")
+    w4 = ops.dev_quantize_w4(gw, 64, True)
+    gx, _ = to_device(ops, rng.standard_normal((M, K), dtype=np.float32), "bf16")
+    want = to_host32(ops, ops.dev_linear_w4(gx, w4))
+    other = np.full((N, K), 3, np_dtype("bf16"))
+    for _ in range(20):
+        ys = [ops.dev_linear_w4(gx, w4) for _ in range(3)]
+        up = ops.gputensor_from_numpy(other)
+        for y in ys:
+            assert np.array_equal(to_host32(ops, y), want)
+        del up
+    assert device_error(0) == 0

@@ -176,3 +176,36 @@ def test_released_workspaces_are_not_in_use(engine):
     calls = [(c, what) for c, _, what in engine.log]
     assert ("free", ptr) in calls and calls.index(("device sync", None)) < calls.index(("free", ptr))
     assert not E._workspaces
+
+
+def _w4(ops, N=6, K=256, group=64, dt=F16):
+    G = -(-K // group)
+    return ops.W4Weight(_fake(ops, (N, K // 8), np.uint32), _fake(ops, (G, N), dt), in_features=K, group=group)
+
+
+def test_unpacked_weight_stays_out_of_the_pool(ops, engine):
+    """More than 64 rows: the 16-bit weight is read by a product that is only
+    queued when the call returns, so its memory must not go back to the pool,
+    where an upload outside the stream's order could take it."""
+    used = {}
+
+    def dequantize(N, K, packed, ldp, scales, zeros, lds, group, sdt, W, wdt, ldw, stream):
+        used["written"] = W
+        return 0
+
+    def gemm(M, N, K, A, lda, ta, B, *rest):
+        used["read"] = B
+        return 0
+
+    value = lambda p: p.value if hasattr(p, "value") else p  # noqa: E731
+    engine.patch("sf_stream_is_capturing", lambda s, out: engine._set(out, 0))
+    engine.patch("sf_dequantize_w4", dequantize)
+    engine.patch("sf_gemm", gemm)
+    engine.patch("sf_gemm_workspace_size", lambda *a: engine._set(a[-1], 6 * 256 * 2))
+    y = ops.dev_linear_w4(_fake(ops, (70, 256), F16), _w4(ops))
+    assert y.shape == (70, 6) and value(used["written"]) == value(used["read"])
+    assert all(p != value(used["read"]) for c, _, p in engine.log if c == "free")
+    assert ops._alloc((6, 256), F16, 0).ptr != value(used["read"])
+    # and it is not the product's own workspace, of the same size here
+    from scaffolding_b200 import engine as E
+    assert sorted(b.ptr for b in E._workspaces.values()).count(value(used["read"])) == 1 and len(E._workspaces) == 2
