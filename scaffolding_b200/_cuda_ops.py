@@ -82,8 +82,9 @@ class CudaBuffer(E.DeviceBuffer):
 def _rebuild_cuda_buffer(arr: np.ndarray, device_id: int = 0):
     buf = _make_buffer(arr.nbytes, device_id)
     with E.on_device(device_id):
-        E.memcpy(buf.ptr, arr.ctypes.data, arr.nbytes, COPY_H2D)
-        E.stream_sync(None)
+        stream = E.upload_stream(device_id)
+        E.memcpy(buf.ptr, arr.ctypes.data, arr.nbytes, COPY_H2D, stream)
+        E.stream_sync(stream)
     return buf
 
 
@@ -147,8 +148,9 @@ def gputensor_from_numpy(arr: np.ndarray, device_id: int = -1) -> GpuTensor:
     gt = _alloc(flat.shape, flat.dtype, dev)
     if flat.nbytes:
         with E.on_device(dev):
-            E.memcpy(gt.ptr, flat.ctypes.data, flat.nbytes, COPY_H2D)
-            E.stream_sync(E.get_stream(dev))
+            stream = E.upload_stream(dev)
+            E.memcpy(gt.ptr, flat.ctypes.data, flat.nbytes, COPY_H2D, stream)
+            E.stream_sync(stream)
     return gt
 
 
@@ -173,9 +175,11 @@ def gputensor_to_device(gt: GpuTensor, target_dev: int) -> GpuTensor:
     if nbytes:
         with E.on_device(gt.device_id):
             E.stream_sync(E.get_stream(gt.device_id))
-        check(lib.sf_memcpy_peer(C.c_void_p(out.ptr), int(target_dev), C.c_void_p(gt.ptr),
-                                 int(gt.device_id), nbytes, None), "sf_memcpy_peer")
-        E.stream_sync(None)
+        with E.on_device(target_dev):
+            stream = E.upload_stream(target_dev)
+            check(lib.sf_memcpy_peer(C.c_void_p(out.ptr), int(target_dev), C.c_void_p(gt.ptr),
+                                     int(gt.device_id), nbytes, stream), "sf_memcpy_peer")
+            E.stream_sync(stream)
     return out
 
 

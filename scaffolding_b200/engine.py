@@ -181,6 +181,14 @@ def stream_capturing(stream: int | None) -> bool:
     return bool(c.value)
 
 
+def upload_stream(dev: int) -> int | None:
+    """Stream of a copy into new memory of ``dev``: the engine's, since the
+    memory may have been an intermediate of work queued there; the legacy one
+    while that is being captured (the copy is no part of the graph)."""
+    stream = get_stream(dev)
+    return None if stream and stream_capturing(stream) else stream
+
+
 def memcpy(dst: int, src: int, nbytes: int, kind: int, stream: int | None = None) -> None:
     check(lib.sf_memcpy(C.c_void_p(dst), C.c_void_p(src), int(nbytes), kind,
                         C.c_void_p(stream) if stream else None), "sf_memcpy")

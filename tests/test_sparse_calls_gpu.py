@@ -85,3 +85,20 @@ def test_upload_beside_an_unpacked_weight(ops, own_stream):
             assert np.array_equal(to_host32(ops, y), want)
         del up
     assert device_error(0) == 0
+
+
+def test_upload_beside_dropped_intermediates(ops, own_stream):
+    """Uploads of the size of an intermediate that queued linears still read."""
+    rng = np.random.default_rng(19)
+    M, K = 4096, 1024
+    gw, _ = to_device(ops, rng.standard_normal((K, K), dtype=np.float32) / np.float32(32), "bf16")
+    gx, _ = to_device(ops, rng.standard_normal((M, K), dtype=np.float32), "bf16")
+    chain = lambda: ops.dev_linear_forward(ops.dev_linear_forward(gx, gw), gw)  # noqa: E731
+    want = to_host32(ops, chain())
+    other = np.full((M, K), 3, np_dtype("bf16"))
+    for _ in range(20):
+        ys = [chain() for _ in range(3)]
+        up = ops.gputensor_from_numpy(other)
+        for y in ys:
+            assert np.array_equal(to_host32(ops, y), want)
+        del up

@@ -209,3 +209,22 @@ def test_unpacked_weight_stays_out_of_the_pool(ops, engine):
     # and it is not the product's own workspace, of the same size here
     from scaffolding_b200 import engine as E
     assert sorted(b.ptr for b in E._workspaces.values()).count(value(used["read"])) == 1 and len(E._workspaces) == 2
+
+
+def test_uploads_keep_the_streams_order(ops, engine):
+    """New memory may be what a dropped intermediate of queued work had: what
+    is copied into it is ordered behind that work, on the engine's stream (and is
+    no part of a graph that is being captured there)."""
+    from scaffolding_b200 import engine as E
+    engine.patch("sf_memcpy", lambda dst, src, n, kind, s: engine.note("copy", s if s is None else getattr(s, "value", s)))
+    engine.patch("sf_memcpy_peer", lambda d, dd, s, sd, n, st: engine.note("copy", getattr(st, "value", st)))
+    for stream, capturing, where in ((None, 0, None), (77, 0, 77), (77, 1, None)):
+        engine.patch("sf_stream_is_capturing", lambda s, out: engine._set(out, capturing))
+        E.set_stream(0, stream)
+        engine.log.clear()
+        ops.gputensor_from_numpy(np.zeros(8, F32), 0)
+        ops._rebuild_cuda_buffer(np.zeros(8, np.uint8), 0)
+        ops.gputensor_to_device(_fake(ops, (8,), dev=1), 0)
+        assert [what for c, _, what in engine.log if c == "copy"] == [where] * 3
+        last = [c for c, _, _ in engine.log if c in ("copy", "sync")]
+        assert last[-1] == "sync" and last.count("sync") >= 3  # the source may be reused when a call returns
