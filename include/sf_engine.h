@@ -413,6 +413,9 @@ int32_t sf_graph_destroy(void* exec);
 /* *capturing = 1 while work on `stream` is being captured, or (the legacy
  * stream) would be refused because another stream is. */
 int32_t sf_stream_is_capturing(void* stream, int32_t* capturing);
+/* *id = a number of the capture that work on `stream` goes into, no two
+ * captures of a process having the same, or 0. */
+int32_t sf_stream_capture_id(void* stream, uint64_t* id);
 
 /* Peer access (_cuda_ops.pyx:550-587). */
 int32_t sf_can_access_peer(int32_t device, int32_t peer, int32_t* can);

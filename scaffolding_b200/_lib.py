@@ -137,6 +137,7 @@ SIGNATURES: dict[str, list] = {
     "sf_graph_launch": [_vp, _vp],
     "sf_graph_destroy": [_vp],
     "sf_stream_is_capturing": [_vp, _P(_i32)],
+    "sf_stream_capture_id": [_vp, _P(C.c_uint64)],
     "sf_can_access_peer": [_i32, _i32, _P(_i32)],
     "sf_enable_peer_access_all": [],
     "sf_device_error_status": [_i32, _P(_i32), _i32],

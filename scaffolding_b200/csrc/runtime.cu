@@ -436,6 +436,21 @@ int32_t sf_stream_is_capturing(void* stream, int32_t* capturing) {
   return SF_OK;
 }
 
+int32_t sf_stream_capture_id(void* stream, uint64_t* id) {
+  if (!id) return fail(SF_ERR_INVALID_ARGUMENT, "null output");
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &st, &n);
+  if (e == cudaErrorStreamCaptureImplicit) {  // the legacy stream, which another's capture closes
+    cudaGetLastError();
+    *id = UINT64_MAX;
+    return SF_OK;
+  }
+  SF_CUDA_TRY(e);
+  *id = st == cudaStreamCaptureStatusNone ? 0 : n;
+  return SF_OK;
+}
+
 int32_t sf_can_access_peer(int32_t device, int32_t peer, int32_t* can) {
   if (!can) return fail(SF_ERR_INVALID_ARGUMENT, "null output");
   int c = 0;

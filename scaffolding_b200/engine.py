@@ -181,6 +181,13 @@ def stream_capturing(stream: int | None) -> bool:
     return bool(c.value)
 
 
+def stream_capture(stream: int | None) -> int:
+    """Number of the capture that work on ``stream`` goes into; 0 for none."""
+    c = C.c_uint64()
+    check(lib.sf_stream_capture_id(stream, C.byref(c)), "sf_stream_capture_id")
+    return c.value
+
+
 def upload_stream(dev: int) -> int | None:
     """Stream of a copy into new memory of ``dev``: the engine's, since the
     memory may have been an intermediate of work queued there; the legacy one
@@ -208,17 +215,28 @@ def stream_sync(stream: int | None) -> None:
 # come, and a buffer that is outgrown is freed.
 workspace_lock = threading.RLock()
 _workspaces: dict[tuple[int, int, str], DeviceBuffer] = {}
+# By capture as well, the newest last.  A graph may be replayed beside other
+# calls on its stream, and as long as it lives: its workspaces are its own.
+_captured: dict[tuple[int, int, str, int], list[DeviceBuffer]] = {}
 
 
 def workspace(dev: int, stream: int | None, nbytes: int, use: str = "sums") -> DeviceBuffer | None:
     """Per-(device, stream, use) scratch buffer, grown on demand; called, and
     its launches queued, with ``workspace_lock`` held.  What a call has in two
     buffers at once are two uses.  It is memory that no allocation can take
-    while queued launches use it: the pool does not know of streams."""
+    while queued launches use it: the pool does not know of streams.  While the
+    stream is being captured the buffer is one of that capture alone, kept
+    until ``release_workspaces(captured=True)``."""
     if nbytes <= 0:
         return None
     key = (dev, int(stream or 0), use)
     with workspace_lock:
+        capture = stream_capture(stream) if stream else 0
+        if capture:
+            bufs = _captured.setdefault(key + (capture,), [])
+            if not bufs or bufs[-1].nbytes < nbytes:
+                bufs.append(DeviceBuffer.alloc(nbytes, dev))
+            return bufs[-1]
         buf = _workspaces.get(key)
         if buf is None or buf.nbytes < nbytes:
             if buf is not None:
@@ -229,15 +247,20 @@ def workspace(dev: int, stream: int | None, nbytes: int, use: str = "sums") -> D
         return buf
 
 
-def release_workspaces() -> None:
-    """Return the workspaces to the pool once nothing queued uses them."""
+def release_workspaces(captured: bool = False) -> None:
+    """Return the workspaces to the pool once nothing queued uses them; with
+    ``captured`` those of captures too, whose graphs must be gone."""
     with workspace_lock:
-        for dev in {key[0] for key in _workspaces}:
+        bufs = list(_workspaces.values())
+        _workspaces.clear()
+        if captured:
+            bufs += [b for held in _captured.values() for b in held]
+            _captured.clear()
+        for dev in {b.device_id for b in bufs}:
             with on_device(dev):
                 check(lib.sf_device_synchronize(), "sf_device_synchronize")
-        for b in _workspaces.values():
+        for b in bufs:
             b.free()
-        _workspaces.clear()
 
 
 # ───────────────────────────── launches ─────────────────────────────

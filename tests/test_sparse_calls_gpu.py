@@ -102,3 +102,74 @@ def test_upload_beside_dropped_intermediates(ops, own_stream):
         for y in ys:
             assert np.array_equal(to_host32(ops, y), want)
         del up
+
+
+class Capture:
+    """``with Capture(ops) as g:`` captures the engine's calls on a stream of
+    its own; ``g.launch()`` replays them there (or on ``stream``)."""
+
+    def __init__(self, ops, stream=None):
+        self.stream = stream or ops.CudaStream(0)
+
+    def __enter__(self):
+        from scaffolding_b200 import engine as E
+        E.set_stream(0, self.stream.cuda_stream)
+        E.check(E.lib.sf_graph_begin(C.c_void_p(self.stream.cuda_stream)), "begin")
+        return self
+
+    def __exit__(self, kind, *exc):
+        from scaffolding_b200 import engine as E
+        self.exe = C.c_void_p()
+        st = E.lib.sf_graph_end(C.c_void_p(self.stream.cuda_stream), C.byref(self.exe))
+        E.set_stream(0, None)
+        if kind is None:
+            E.check(st, "end")
+
+    def launch(self, stream=None):
+        from scaffolding_b200 import engine as E
+        E.check(E.lib.sf_graph_launch(self.exe, C.c_void_p((stream or self.stream).cuda_stream)), "launch")
+
+    def destroy(self):
+        from scaffolding_b200 import engine as E
+        E.check(E.lib.sf_graph_destroy(self.exe), "destroy")
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_captured_workspaces(gpu, ops, dt):
+    """Two graphs captured on one stream, whose products keep sums or operand
+    panels in a workspace, replayed side by side and beside direct calls of the
+    stream with a larger one."""
+    from oracle import oracle as O
+    from scaffolding_b200 import engine as E
+    rng = np.random.default_rng(23)
+    K, N = 4096, 256
+    gw, w = to_device(ops, rng.standard_normal((N, K), dtype=np.float32) / np.float32(64), dt)
+    xs = [to_device(ops, rng.standard_normal((M, K), dtype=np.float32), dt) for M in (64, 64, 256)]
+    s1, s2 = ops.CudaStream(0), ops.CudaStream(0)
+    graphs, ys = [], []
+    for gx, _ in xs[:2]:
+        with Capture(ops, s1) as g:
+            ys.append(ops.dev_linear_forward(gx, gw))
+        graphs.append(g)
+    assert len(E._captured) >= 2
+    E.set_stream(0, s1.cuda_stream)
+    try:
+        for _ in range(10):
+            graphs[0].launch(s1)
+            graphs[1].launch(s2)
+            big = ops.dev_linear_forward(xs[2][0], gw)
+        ops.empty_cache()
+        for g, s in zip(graphs, (s2, s1)):
+            g.launch(s)
+        ops.device_synchronize()
+    finally:
+        E.set_stream(0, None)
+    for y, (_, x) in zip(ys + [big], xs):
+        ref = x.astype(np.float64) @ w.astype(np.float64).T
+        # 2 K operations of the sum, the output's rounding, 3xTF32 for fp32
+        tol = 2.0 ** -22 * K * (np.abs(x).astype(np.float64) @ np.abs(w).T) + 2.0 ** -8 * (dt == "bf16") * np.abs(ref)
+        assert (np.abs(to_host32(ops, y) - ref) <= tol).all()
+    for g in graphs:
+        g.destroy()
+    E.release_workspaces(captured=True)
+    assert device_error(0) == 0

@@ -49,6 +49,8 @@ class _Engine:
         self.patch("sf_set_device", lambda dev: 0)
         self.patch("sf_device_synchronize", lambda: self.note("device sync", None))
         self.patch("sf_stream_synchronize", lambda s: self.note("sync", s))
+        if hasattr(lib, "sf_stream_capture_id"):
+            self.patch("sf_stream_capture_id", lambda s, out: self._set(out, self.capture_id.get(s, 0)))
 
     @staticmethod
     def _set(out, value):
@@ -81,6 +83,8 @@ class _Engine:
 def engine(monkeypatch):
     from scaffolding_b200 import engine as E
     monkeypatch.setattr(E, "_workspaces", {})
+    if hasattr(E, "_captured"):
+        monkeypatch.setattr(E, "_captured", {})
     monkeypatch.setattr(E, "_streams", {})
     return _Engine(monkeypatch)
 
@@ -228,3 +232,26 @@ def test_uploads_keep_the_streams_order(ops, engine):
         assert [what for c, _, what in engine.log if c == "copy"] == [where] * 3
         last = [c for c, _, _ in engine.log if c in ("copy", "sync")]
         assert last[-1] == "sync" and last.count("sync") >= 3  # the source may be reused when a call returns
+
+
+def test_captures_have_workspaces_of_their_own(engine):
+    """A graph uses its workspaces at every replay, beside other calls and
+    graphs of the stream it was captured on: none is another's, and none is
+    freed for a larger one or by empty_cache."""
+    from scaffolding_b200 import engine as E
+    ws = lambda n: E.workspace(0, 77, n).ptr  # noqa: E731
+    direct = ws(1000)
+    engine.capture_id[77] = 5
+    first = [ws(1000), ws(1000), ws(9000)]
+    engine.capture_id[77] = 6
+    second = ws(1000)
+    engine.capture_id[77] = 0
+    assert ws(1000) == direct and first[0] == first[1]
+    assert len({direct, first[0], first[2], second}) == 4
+    ws(50000)  # the stream's own grows
+    E.release_workspaces()
+    freed = [what for c, _, what in engine.log if c == "free"]
+    assert direct in freed and not {first[0], first[2], second} & set(freed)
+    E.release_workspaces(captured=True)
+    freed = [what for c, _, what in engine.log if c == "free"]
+    assert {first[0], first[2], second} <= set(freed)
