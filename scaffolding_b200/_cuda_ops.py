@@ -294,19 +294,21 @@ def dev_batched_matmul_nt(gt_a: GpuTensor, gt_b: GpuTensor) -> GpuTensor:
 
 
 def dev_linear_forward(gt_x: GpuTensor, gt_weight: GpuTensor, gt_bias: GpuTensor | None = None,
-                       activation: str = "none", out_dtype=None) -> GpuTensor:
+                       activation: str = "none", out_dtype=None, out: GpuTensor | None = None) -> GpuTensor:
     """y = act(x @ W^T + bias) with bias and activation fused into the GEMM
     epilogue (``_cuda_ops.pyx:1278-1302``; activation was a separate launch,
-    ``nn/functional.py:37-40``)."""
+    ``nn/functional.py:37-40``).  ``out``: the result's buffer, which shares no
+    memory with the operands."""
     _check_pair(gt_x, gt_weight)
     K = gt_x.shape[-1]
     M = int(np.prod(gt_x.shape[:-1], dtype=np.int64))
     N, Kw = gt_weight.shape
     if Kw != K:
         raise ValueError(f"linear shape mismatch: x {gt_x.shape}, W {gt_weight.shape}")
-    odt = _out_dtype(gt_x, out_dtype)
+    _apart(out, gt_x, gt_weight, gt_bias)
+    odt = _out_dtype(gt_x, out_dtype if out is None else out.dtype)
     dev = gt_x.device_id
-    y = _alloc(gt_x.shape[:-1] + (N,), odt, dev)
+    y = _result(out, gt_x.shape[:-1] + (N,), odt, dev, "out")
     bias_ptr, bias_dt = 0, DT_F32
     if gt_bias is not None:
         if gt_bias.numel != N:
@@ -468,6 +470,13 @@ class MoeRoute:
         self.scratch = None  # per-block counts, kept with the buffers they are used with
 
 
+def moe_route_scratch(tokens: int, experts: int, top_k: int) -> int:
+    """Bytes of counts that routing so many tokens takes (0 for few)."""
+    need = C.c_size_t()
+    check(lib.sf_moe_route_workspace_size(tokens, experts, top_k, C.byref(need)), "sf_moe_route_workspace_size")
+    return need.value
+
+
 def dev_moe_route(gt_logits: GpuTensor, top_k: int, renormalize: bool = True,
                   out: MoeRoute | None = None) -> MoeRoute:
     """Route ``[tokens, experts]`` logits (fp32 / bf16 / fp16): the ``top_k``
@@ -484,8 +493,7 @@ def dev_moe_route(gt_logits: GpuTensor, top_k: int, renormalize: bool = True,
     k = int(top_k)
     dev = gt_logits.device_id
     code = E.dtype_code(gt_logits.dtype)
-    need = C.c_size_t()
-    check(lib.sf_moe_route_workspace_size(T, X, k, C.byref(need)), "sf_moe_route_workspace_size")
+    need = moe_route_scratch(T, X, k)
     if out is None:
         i32 = np.int32
         out = MoeRoute(_alloc((T, k), i32, dev), _alloc((T, k), np.float32, dev),
@@ -495,14 +503,13 @@ def dev_moe_route(gt_logits: GpuTensor, top_k: int, renormalize: bool = True,
         for name, shape in (("experts", (T, k)), ("weights", (T, k)), ("offsets", (X + 1,)),
                             ("rows", (T * k,)), ("slots", (T, k))):
             _result(getattr(out, name), shape, _F32 if name == "weights" else _I32, dev, name)
-    if need.value and (out.scratch is None or out.scratch.nbytes < need.value
-                       or out.scratch.device_id != dev):
-        out.scratch = _make_buffer(need.value, dev)
-    ws = out.scratch.ptr if need.value else None
+    if need and (out.scratch is None or out.scratch.nbytes < need or out.scratch.device_id != dev):
+        out.scratch = _make_buffer(need, dev)
+    ws = out.scratch.ptr if need else None
     with E.on_device(dev):
         check(lib.sf_moe_route(T, X, k, _ptr(gt_logits), code, X, 1 if renormalize else 0,
                                _ptr(out.experts), _ptr(out.weights), _ptr(out.offsets),
-                               _ptr(out.rows), _ptr(out.slots), ws, need.value, E.get_stream(dev)),
+                               _ptr(out.rows), _ptr(out.slots), ws, need, E.get_stream(dev)),
               "sf_moe_route")
     return out
 

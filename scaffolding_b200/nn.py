@@ -130,9 +130,9 @@ class Linear4:
         if self.bias is not None and self.bias.device_id != dev:
             self.bias = ops.gputensor_to_device(self.bias, dev)
 
-    def forward(self, x: GpuTensor, activation: str = "none") -> GpuTensor:
+    def forward(self, x: GpuTensor, activation: str = "none", out: GpuTensor | None = None) -> GpuTensor:
         self._to(x.device_id)
-        return ops.dev_linear_w4(x, self.weight, self.bias, activation)
+        return ops.dev_linear_w4(x, self.weight, self.bias, activation, out=out)
 
     __call__ = forward
 
@@ -176,23 +176,53 @@ class MoE:
             setattr(self, name, ops.gputensor_astype(w, dtype) if dtype is not None else w)
         return self
 
-    def forward(self, x: GpuTensor, residual: GpuTensor | None = None) -> GpuTensor:
+    def forward(self, x: GpuTensor, residual: GpuTensor | None = None,
+                out: GpuTensor | None = None) -> GpuTensor:
         """``x [..., dim]`` to the same shape; ``residual`` (that shape too)
-        is added to the experts' sum before it is rounded."""
+        is added to the experts' sum before it is rounded.  ``out``: the
+        result's buffer, which may be ``x`` or ``residual``.  What the steps hand
+        to each other lies in the stream's workspace, or in one of the
+        graph's own while the stream is being captured."""
         if x.ndim < 1 or x.shape[-1] != self.dim:
             raise ValueError(f"MoE of width {self.dim}: x {x.shape}")
         if self.router.device_id != x.device_id:
             self.to(x.device_id)
         if residual is not None and residual.shape != x.shape:
             raise ValueError(f"residual must be {x.shape}, got {residual.shape}")
+        o = ops._result(out, x.shape, x.dtype, x.device_id, "out")
         flat = ops.dev_reshape(x, (math.prod(x.shape[:-1]), self.dim))
-        logits = ops.dev_linear_forward(flat, self.router, out_dtype=np.float32)
-        route = ops.dev_moe_route(logits, self.top_k, self.renormalize)
-        h = ops.dev_grouped_linear(flat, self.up, route.offsets, activation=self.activation,
-                                   rows=route.rows)
-        y = ops.dev_grouped_linear(h, self.down, route.offsets)
         res = ops.dev_reshape(residual, flat.shape) if residual is not None else None
-        return ops.dev_reshape(ops.dev_moe_combine(y, route.slots, route.weights, res), x.shape)
+        with E.workspace_lock:
+            logits, route, h, y = self._between(flat)
+            ops.dev_linear_forward(flat, self.router, out=logits)
+            ops.dev_moe_route(logits, self.top_k, self.renormalize, out=route)
+            ops.dev_grouped_linear(flat, self.up, route.offsets, activation=self.activation,
+                                   rows=route.rows, out=h)
+            ops.dev_grouped_linear(h, self.down, route.offsets, out=y)
+            ops.dev_moe_combine(y, route.slots, route.weights, res, out=ops.dev_reshape(o, flat.shape))
+        return o
+
+    def _between(self, flat: GpuTensor):
+        """Logits, route and the two products' results for tokens ``flat``,
+        one after the other in the workspace."""
+        T, k, dev = flat.shape[0], self.top_k, flat.device_id
+        X, wide = self.up.shape[:2]
+        hidden = wide // 2 if E.grouped_act_code(self.activation) == E.ACT_SILU_GATE else wide
+        f32, i32 = np.float32, np.int32
+        counts = ops.moe_route_scratch(T, X, k)
+        shapes = [((T, X), f32), ((T, k), i32), ((T, k), f32), ((X + 1,), i32), ((T * k,), i32), ((T, k), i32),
+                  ((T * k, hidden), flat.dtype), ((T * k, self.down.shape[1]), flat.dtype), ((counts,), np.uint8)]
+        sizes = [math.prod(shape) * np.dtype(dt).itemsize for shape, dt in shapes]
+        starts = [0]
+        for size in sizes:
+            starts.append(starts[-1] + -(-size // 256) * 256)
+        base = E.workspace(dev, E.get_stream(dev), starts[-1], "layer").ptr
+        logits, *parts, h, y, scratch = (
+            GpuTensor(ops.CudaBuffer(base + at, size, dev, False), shape, dt, dev)
+            for at, size, (shape, dt) in zip(starts, sizes, shapes))
+        route = ops.MoeRoute(*parts)
+        route.scratch = scratch.buffer
+        return logits, route, h, y
 
     __call__ = forward
 

@@ -173,3 +173,55 @@ def test_captured_workspaces(gpu, ops, dt):
         g.destroy()
     E.release_workspaces(captured=True)
     assert device_error(0) == 0
+
+
+@pytest.mark.parametrize("T", [3, 300])
+def test_captured_moe_layer(gpu, ops, T):
+    """A captured nn.MoE replayed after direct calls, uploads and allocations
+    of the sizes of everything between its steps: the bits of the direct call,
+    and nothing of what was allocated since is written."""
+    from scaffolding_b200 import engine as E
+    from scaffolding_b200 import nn
+    rng = np.random.default_rng(T)
+    dim, hidden, X, k = 64, 96, 12, 3
+    bf = np_dtype("bf16")
+    m = nn.MoE(dim, hidden, X, k, device=0, dtype=bf, rng=rng)
+    gx, _ = to_device(ops, rng.standard_normal((T, dim), dtype=np.float32), "bf16")
+    out = ops._alloc((T, dim), bf, 0)
+    want = to_host32(ops, m(gx, gx))
+    with Capture(ops) as g:
+        m(gx, gx, out=out)
+    X1 = X + 1
+    guards = [ops.gputensor_from_numpy(np.full(n, 77, np.uint8))
+              for n in (T * X * 4, T * k * 4, T * k * 4, X1 * 4, T * k * hidden * 2, T * k * dim * 2) for _ in range(3)]
+    other, _ = to_device(ops, rng.standard_normal((T, dim), dtype=np.float32), "bf16")
+    for _ in range(3):
+        m(other)
+        g.launch()
+        g.stream.synchronize()
+        assert np.array_equal(to_host32(ops, out), want)
+    for t in guards:
+        assert (ops.gputensor_to_numpy(t) == 77).all()
+    g.destroy()
+    E.release_workspaces(captured=True)
+    assert device_error(0) == 0
+
+
+def test_moe_layers_of_two_threads(gpu, ops):
+    """Two layers in two threads on the default stream: the bits of the same
+    calls made one by one."""
+    from scaffolding_b200 import nn
+    rng = np.random.default_rng(2)
+    bf = np_dtype("bf16")
+    jobs = []
+    for T in (40, 700):
+        m = nn.MoE(64, 96, 12, 3, device=0, dtype=bf, rng=rng)
+        gx, _ = to_device(ops, rng.standard_normal((T, 64), dtype=np.float32), "bf16")
+        jobs.append((m, gx, to_host32(ops, m(gx))))
+
+    def loop(m, gx, want):
+        for _ in range(60):
+            assert np.array_equal(to_host32(ops, m(gx)), want)
+
+    _in_threads(*[lambda j=j: loop(*j) for j in jobs])
+    assert device_error(0) == 0

@@ -255,3 +255,63 @@ def test_captures_have_workspaces_of_their_own(engine):
     E.release_workspaces(captured=True)
     freed = [what for c, _, what in engine.log if c == "free"]
     assert {first[0], first[2], second} <= set(freed)
+
+
+def _moe_engine(engine):
+    """Records what the four steps of nn.MoE write: (step, address)."""
+    value = lambda p: getattr(p, "value", p)  # noqa: E731
+    wrote = []
+
+    def note(step, *ptrs):
+        wrote.extend((step, value(p)) for p in ptrs)
+        return 0
+
+    engine.patch("sf_stream_is_capturing", lambda s, out: engine._set(out, 1 if engine.capture_id.get(s) else 0))
+    engine.patch("sf_gemm_workspace_size", lambda *a: engine._set(a[-1], 0))
+    engine.patch("sf_gemm", lambda M, N, K, A, lda, ta, B, ldb, tb, Cp, *r: note("logits", Cp))
+    engine.patch("sf_moe_route", lambda T, X, k, z, dt, ld, rn, e, w, o, r, s, ws, n, st: note("route", e, w, o, r, s, ws))
+    _grouped_needs(engine, lambda M: 0)
+    engine.patch("sf_gemm_grouped", lambda *a: note("product", a[15]))
+    engine.patch("sf_moe_combine", lambda *a: note("combine", a[11]))
+    return wrote
+
+
+def test_moe_intermediates_stay_out_of_the_pool(ops, engine):
+    """What nn.MoE's steps hand to each other is read by launches that are only
+    queued, or captured, when it returns: none of that memory goes back to the
+    pool, and a capture's is not that of later direct calls."""
+    from scaffolding_b200 import engine as E
+    from scaffolding_b200 import nn
+    wrote = _moe_engine(engine)
+    m = _moe(ops, nn, dtype=F16)
+    E.set_stream(0, 77)
+    engine.capture_id[77] = 3
+    held = m(_fake(ops, (300, 64), F16))
+    captured = {p for step, p in wrote if step != "combine"}
+    assert len(captured) == 9 and 0 not in captured  # logits, five of the route and its counts, two products
+    assert not [p for c, _, p in engine.log if c == "free" and p in captured]
+    engine.capture_id[77] = 0
+    wrote.clear()
+    m(_fake(ops, (300, 64), F16))
+    m(_fake(ops, (2000, 64), F16))
+    assert not captured & {p for _, p in wrote} and held.shape == (300, 64)
+    spans = [(b.ptr, b.ptr + b.nbytes) for bufs in E._captured.values() for b in bufs]
+    assert all(any(lo <= p < hi for lo, hi in spans) for p in captured)
+
+
+def test_modules_write_into_kept_results(ops, engine):
+    """out= of nn.MoE and nn.Linear4, and its refusals."""
+    from scaffolding_b200 import nn
+    wrote = _moe_engine(engine)
+    m = _moe(ops, nn, dtype=F16)
+    out = ops.GpuTensor(ops.CudaBuffer(512, 2 * 20 * 64, 0, False), (4, 5, 64), F16, 0)
+    x = ops.GpuTensor(ops.CudaBuffer(1 << 16, 2 * 20 * 64, 0, False), (4, 5, 64), F16, 0)
+    assert m(x, out=out) is out and wrote[-1] == ("combine", 512)
+    assert m(x, x, out=x) is x and wrote[-1] == ("combine", 1 << 16)
+    for bad in (_fake(ops, (20, 64), F16), _fake(ops, (4, 5, 64))):
+        with pytest.raises(ValueError, match="out must be"):
+            m(x, out=bad)
+    engine.patch("sf_linear_w4", lambda *a: engine.note("y", a[13]))
+    lin = nn.Linear4(_w4(ops, N=64))
+    x = ops.GpuTensor(ops.CudaBuffer(1 << 16, 4096, 0, False), (4, 5, 256), F16, 0)
+    assert lin(x, out=out) is out and engine.log[-1][2] == 512
