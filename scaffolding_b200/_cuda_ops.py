@@ -435,10 +435,18 @@ def _result(out, shape, dtype, dev, name: str) -> GpuTensor:
     return out
 
 
-def _apart(out, *inputs) -> None:
-    """Refuses a result buffer that is an input's."""
-    if out is not None and out.numel and any(t is not None and t.buffer is out.buffer for t in inputs):
-        raise ValueError("out must not share memory with the inputs")
+def _apart(one, *others) -> None:
+    """Refuses a result that shares memory with an input, by address (``one``
+    is the result, or the input of several results)."""
+    if one is None or not one.numel:
+        return
+    mine = one.buffer
+    lo, hi = mine.ptr, mine.ptr + mine.nbytes
+    for t in others:
+        if t is not None:
+            b = t.buffer
+            if b is mine or (b.ptr < hi and lo < b.ptr + b.nbytes):
+                raise ValueError("out must not share memory with the inputs")
 
 
 def _int32(t: GpuTensor, name: str) -> GpuTensor:
@@ -485,7 +493,8 @@ def dev_moe_route(gt_logits: GpuTensor, top_k: int, renormalize: bool = True,
     ``renormalize=False`` -- and the choices grouped by expert for
     ``dev_grouped_linear`` (``sf_moe_route``).  ``out``: a MoeRoute whose
     buffers are written instead of new ones (a captured graph, a decoding
-    loop); it must not be read by work in flight on another stream.  New (the
+    loop), which share no memory with the logits; it must not be read by work in
+    flight on another stream.  New (the
     reference has no routed layers)."""
     if gt_logits.ndim != 2:
         raise ValueError(f"router logits must be [tokens, experts], got {gt_logits.shape}")
@@ -503,6 +512,7 @@ def dev_moe_route(gt_logits: GpuTensor, top_k: int, renormalize: bool = True,
         for name, shape in (("experts", (T, k)), ("weights", (T, k)), ("offsets", (X + 1,)),
                             ("rows", (T * k,)), ("slots", (T, k))):
             _result(getattr(out, name), shape, _F32 if name == "weights" else _I32, dev, name)
+        _apart(gt_logits, out.experts, out.weights, out.offsets, out.rows, out.slots)
     if need and (out.scratch is None or out.scratch.nbytes < need or out.scratch.device_id != dev):
         out.scratch = _make_buffer(need, dev)
     ws = out.scratch.ptr if need else None
@@ -527,7 +537,8 @@ def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTen
     ``bias`` ``[experts, N]``.  ``activation="silu_gate"`` takes ``[experts,
     2 N, K]``, the first N rows the gate: ``silu(gate) * value``.  The group
     sizes stay on the device.  Rows of the result in no group are not written
-    (``dev_moe_route``'s offsets cover every row)."""
+    (``dev_moe_route``'s offsets cover every row).  ``out`` shares no memory
+    with the inputs."""
     act = E.grouped_act_code(activation)
     if gt_x.ndim != 2 or gt_weight.ndim != 3:
         raise ValueError(f"grouped linear shapes: x {gt_x.shape}, weight {gt_weight.shape}")
@@ -547,7 +558,7 @@ def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTen
     N = wide // 2 if act == ACT_SILU_GATE else wide
     M = rows.shape[0] if rows is not None else gt_x.shape[0]
     dev = _same_device(gt_x, gt_weight, gt_offsets, gt_bias, rows, out)
-    _apart(out, gt_x, gt_weight, gt_bias)
+    _apart(out, gt_x, gt_weight, gt_bias, gt_offsets, rows)
     odt = _out_dtype(gt_x, out_dtype if out is None else out.dtype)
     y = _result(out, (M, N), odt, dev, "out")
     bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
@@ -580,7 +591,7 @@ def dev_moe_combine(gt_y: GpuTensor, gt_slots: GpuTensor, gt_weights: GpuTensor,
     ``residual[t] + sum_j weights[t, j] * y[slots[t, j]]`` in fp32, rounded
     once; ``slots`` and ``weights`` as in a MoeRoute, ``y`` ``[slots, C]``.
     A slot outside ``y`` (-1, say, for a dropped choice) adds nothing.  ``out``
-    may be ``residual``, not ``y``."""
+    may be ``residual``, and shares no memory with the other inputs."""
     if gt_y.ndim != 2 or gt_slots.ndim != 2:
         raise ValueError(f"combine shapes: y {gt_y.shape}, slots {gt_slots.shape}")
     T, k = _int32(gt_slots, "slots").shape
@@ -590,7 +601,8 @@ def dev_moe_combine(gt_y: GpuTensor, gt_slots: GpuTensor, gt_weights: GpuTensor,
     if residual is not None and (residual.shape != (T, width) or residual.dtype != gt_y.dtype):
         raise ValueError(f"residual must be {(T, width)} {gt_y.dtype}, got {residual.shape} {residual.dtype}")
     dev = _same_device(gt_y, gt_slots, gt_weights, residual, out)
-    _apart(out, gt_y)
+    _apart(out, gt_y, gt_slots, gt_weights,
+           None if out is None or residual is None or residual.ptr == out.ptr else residual)
     o = _result(out, (T, width), gt_y.dtype, dev, "out")
     with E.on_device(dev):
         check(lib.sf_moe_combine(T, width, k, _ptr(gt_y), gt_y.shape[0], width,
@@ -733,7 +745,7 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
     stream's workspace and run the GEMM.  During a graph capture more rows run
     64 at a time on ``sf_linear_w4`` instead: a graph must not hold the
     dequantised weight, whose memory the stream's next call uses again.
-    ``out`` shares no memory with x."""
+    ``out`` shares no memory with x, the bias or the weight."""
     act = E.act_code(activation)
     if gt_x.dtype != weight.scales.dtype:
         raise TypeError(f"x and the weight's scales must share a dtype ({gt_x.dtype} vs {weight.scales.dtype})")
@@ -746,7 +758,7 @@ def dev_linear_w4(gt_x: GpuTensor, weight: W4Weight, gt_bias: GpuTensor | None =
         raise ValueError(f"bias has {gt_bias.numel} elements, expected {n}")
     M = int(math.prod(gt_x.shape[:-1]))
     dev = _same_device(gt_x, weight.packed, gt_bias, out)
-    _apart(out, gt_x, gt_bias)
+    _apart(out, gt_x, gt_bias, weight.packed, weight.scales, weight.zeros)
     odt = _out_dtype(gt_x, out_dtype if out is None else out.dtype)
     y = _result(out, gt_x.shape[:-1] + (n,), odt, dev, "out")
     bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32

@@ -315,3 +315,56 @@ def test_modules_write_into_kept_results(ops, engine):
     lin = nn.Linear4(_w4(ops, N=64))
     x = ops.GpuTensor(ops.CudaBuffer(1 << 16, 4096, 0, False), (4, 5, 256), F16, 0)
     assert lin(x, out=out) is out and engine.log[-1][2] == 512
+
+
+def _at(ops, lo, shape, dtype=F32):
+    n = int(np.prod(shape)) * np.dtype(dtype).itemsize
+    return ops.GpuTensor(ops.CudaBuffer(lo, n, 0, False), shape, dtype, 0)
+
+
+def test_results_share_no_memory_with_any_input(ops):
+    """By address: views of one allocation are different buffers."""
+    from scaffolding_b200.parallel import row_slice
+    share = pytest.raises(ValueError, match="share memory")
+    # rows 8.. of an allocation as the result, rows 0..11 as the input
+    whole = _at(ops, 4096, (24, 16), F16)
+    x, out = row_slice(whole, 0, 12), row_slice(whole, 8, 20)
+    w, off = _at(ops, 1 << 20, (2, 16, 16), F16), _at(ops, 1 << 21, (3,), I32)
+    with share:
+        ops.dev_grouped_linear(x, w, off, out=out)
+    y = _at(ops, 4096, (12, 16), F16)
+    for name, t in (("offsets", _at(ops, 4096 + 32, (3,), I32)), ("bias", _at(ops, 4096, (2, 16), F16)),
+                    ("rows", _at(ops, 4096 + 300, (12,), I32)), ("weight", _at(ops, 4096, (2, 16, 16), F16))):
+        with share:
+            ops.dev_grouped_linear(_at(ops, 1 << 19, (12, 16), F16), t if name == "weight" else w,
+                                   t if name == "offsets" else off, t if name == "bias" else None,
+                                   rows=t if name == "rows" else None, out=y)
+    s, p = _at(ops, 1 << 20, (4, 3), I32), _at(ops, 1 << 21, (4, 3))
+    e = _at(ops, 4096, (4, 16))
+    for args in ((_at(ops, 4000, (12, 16)), s, p), (_at(ops, 1 << 18, (12, 16)), _at(ops, 4096, (4, 3), I32), p),
+                 (_at(ops, 1 << 18, (12, 16)), s, _at(ops, 4100, (4, 3)))):
+        with share:
+            ops.dev_moe_combine(*args, out=e)
+    with share:  # a residual is the result's memory or none of it
+        ops.dev_moe_combine(_at(ops, 1 << 18, (12, 16)), s, p, _at(ops, 4096 + 64, (4, 16)), out=e)
+    z = _at(ops, 4096, (4, 128), F16)
+    packed, scales, zeros = _at(ops, 1 << 20, (128, 16), np.uint32), _at(ops, 1 << 21, (2, 128), F16), None
+    for name, t in (("packed", _at(ops, 4090, (128, 16), np.uint32)), ("scales", _at(ops, 4096, (2, 128), F16)),
+                    ("zeros", _at(ops, 4608, (2, 128), F16)), ("x", _at(ops, 4096 + 1000, (4, 128), F16))):
+        w4 = ops.W4Weight(t if name == "packed" else packed, t if name == "scales" else scales,
+                          t if name == "zeros" else zeros, in_features=128, group=64)
+        with share:
+            ops.dev_linear_w4(t if name == "x" else _at(ops, 1 << 18, (4, 128), F16), w4, out=z)
+    r = ops.MoeRoute(_at(ops, 1 << 20, (4, 2), I32), _at(ops, 1 << 21, (4, 2)), _at(ops, 1 << 22, (9,), I32),
+                     _at(ops, 4096, (8,), I32), _at(ops, 1 << 23, (4, 2), I32))
+    with share:
+        ops.dev_moe_route(_at(ops, 4096 + 16, (4, 8)), 2, out=r)
+
+
+def test_result_next_to_an_input(ops, engine):
+    """Neighbours in one allocation are apart."""
+    engine.patch("sf_moe_combine", lambda *a: engine.note("combine", a[11]))
+    e = _at(ops, 4096, (4, 16))
+    args = _at(ops, 4096 + 256, (12, 16)), _at(ops, 4096 - 48, (4, 3), I32), _at(ops, 1 << 21, (4, 3))
+    assert ops.dev_moe_combine(*args, out=e) is e
+    assert ops.dev_moe_combine(*args, _at(ops, 4096, (4, 16)), out=e) is e
