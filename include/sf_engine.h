@@ -198,7 +198,8 @@ int32_t sf_gemm_grouped_workspace_size(int64_t groups, int64_t M, int64_t N, int
  *   slot p of offsets[e] <= p < offsets[e + 1] holds token rows[p], by rising
  *   token; slots[t][j] is the slot of choice j of token t.
  * expert_ids, weights and slots are [tokens][top_k], rows [tokens * top_k],
- * offsets [experts + 1].  At most 1024 experts and top_k 32.  The same
+ * offsets [experts + 1].  At most 1024 experts, top_k 32 and tokens * top_k
+ * of 2^31 - 2^23 - 1.  The same
  * inputs give the same bits.  The workspace (0 bytes for few tokens) is free
  * again when the call's kernels are done.  No counterpart in the reference. */
 int32_t sf_moe_route_workspace_size(int64_t tokens, int64_t experts, int32_t top_k, size_t* bytes);

@@ -40,6 +40,10 @@ namespace {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 32;
+// Token and choice numbers are 32 bits.  What is added to one past the last
+// (the end of a block's chunk, at most 2^22 tokens; a warp's stride) stays in
+// range with this many.
+constexpr int64_t kMostChoices = INT32_MAX - (1 << 23);
 constexpr int kSmallTokens = 256;
 constexpr int kRouteThreads = 512;
 constexpr int kSmallThreads = 1024;
@@ -481,8 +485,8 @@ int32_t check_route(int64_t tokens, int64_t experts, int32_t top_k) {
   if (experts > kMaxExperts || top_k > kMaxTopK)
     return fail(SF_ERR_UNSUPPORTED, "top_k %d of %lld experts (at most %d of %d)", top_k,
                 (long long)experts, kMaxTopK, kMaxExperts);
-  if (tokens > INT32_MAX / top_k)
-    return fail(SF_ERR_UNSUPPORTED, "%lld tokens with %d choices exceed 2^31-1 slots",
+  if (tokens > kMostChoices / top_k)
+    return fail(SF_ERR_UNSUPPORTED, "%lld tokens with %d choices exceed 2^31-2^23-1 slots",
                 (long long)tokens, top_k);
   return SF_OK;
 }

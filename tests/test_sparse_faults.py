@@ -368,3 +368,21 @@ def test_result_next_to_an_input(ops, engine):
     args = _at(ops, 4096 + 256, (12, 16)), _at(ops, 4096 - 48, (4, 3), I32), _at(ops, 1 << 21, (4, 3))
     assert ops.dev_moe_combine(*args, out=e) is e
     assert ops.dev_moe_combine(*args, _at(ops, 4096, (4, 16)), out=e) is e
+
+
+def test_route_leaves_room_for_its_index_arithmetic():
+    """A block's chunk of up to 2^22 tokens may end past the last token: that
+    end is a 32-bit number too."""
+    import ctypes as C
+
+    from scaffolding_b200._lib import SF_ERR_UNSUPPORTED as NO, lib
+    sz = C.c_size_t()
+    most = (1 << 31) - (1 << 23) - 1
+    for k in (1, 2, 32):
+        assert lib.sf_moe_route_workspace_size(most // k, 64, k, C.byref(sz)) == 0
+        for tokens in (most // k + 1, ((1 << 31) - 1) // k):
+            assert lib.sf_moe_route_workspace_size(tokens, 64, k, C.byref(sz)) == NO
+    assert lib.sf_moe_route_workspace_size(most, 64, 1, C.byref(sz)) == 0
+    blocks = sz.value // (64 * 4)
+    chunk = -(-most // 512)
+    assert blocks == -(-most // chunk) and blocks * chunk + 16 * 4 < 1 << 31
