@@ -225,3 +225,171 @@ def test_moe_layers_of_two_threads(gpu, ops):
 
     _in_threads(*[lambda j=j: loop(*j) for j in jobs])
     assert device_error(0) == 0
+
+
+# ───────────── sizes at which rings, clusters and accumulators come round ─────────────
+# The expected launch is worked out from the sizes by the rules of the dispatch: rows
+# per group choose the tile, tiles and k-blocks the cluster.
+
+SMS = 148
+
+
+def grouped_plan(X, M, K, N, gate):
+    """(rows of a tile, CTAs that share one, most tiles, k-blocks)."""
+    few = M <= 16 * X
+    bn = (32 if gate else 64) if few else (128 if gate else 256)
+    most, kb = (M // bn + min(X, M)) * -(-N // 128), -(-K // 64)
+    splits = 1
+    while few and splits < 8 and kb >= 8 * splits and most * splits * 2 <= (
+            SMS if splits == 1 else SMS * 3 // 4 if splits == 2 else SMS // 3):
+        splits *= 2
+    return bn, splits, most, kb
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("X,M,K,N,act,gather,splits", [
+    (8, 2, 512, 300, "none", 1, 2),        # eight k-blocks, three weight blocks
+    (2, 5, 520, 2000, "silu", None, 2),    # 9 = 5 + 4 k-blocks, the last of 8 columns
+    (1, 1, 1024, 128, "none", None, 4),    # one tile
+    (3, 40, 1096, 500, "gelu_tanh", 7, 4), # 18 k-blocks in shares of 5: 3 for the last
+    (4, 9, 2048, 100, "none", 9, 8),
+    (1, 16, 2112, 500, "silu", None, 8),   # 33 k-blocks in shares of 5: none for the last rank
+    (2, 31, 4104, 260, "none", 3, 8),      # 65 in shares of 9
+    (1, 1, 512, 1000, "silu_gate", 1, 2),
+    (2, 20, 1032, 300, "silu_gate", None, 4),
+    (1, 13, 2112, 140, "silu_gate", 13, 8),
+    (2, 30, 2104, 20, "silu_gate", 8, 8),
+])
+def test_grouped_clusters(gpu, ops, dt, X, M, K, N, act, gather, splits):
+    """A tile's k-blocks shared by two, four and eight CTAs: uneven shares, a
+    rank without any, K no multiple of 64."""
+    from tests.test_moe_gpu import assert_within, run_grouped
+    assert grouped_plan(X, M, K, N, act == "silu_gate")[1] == splits
+    rng = np.random.default_rng(K + N)
+    for bias in (False, True):
+        assert_within(*run_grouped(ops, rng, dt, X, M, K, N, act, bias, gather), f"{X} {M} {K} {N} {act}")
+    assert device_error(0) == 0
+
+
+@pytest.mark.parametrize("X,M,K,N,act,gather,bn", [
+    (64, 256, 640, 1000, "silu_gate", 40, 32),     # narrow gated: 10 k-blocks in a ring of five
+    (64, 700, 576, 1100, "none", None, 64),        # narrow: 9 in a ring of eight
+    (64, 1000, 704, 1100, "gelu_tanh", 300, 64),
+    (3, 900, 712, 4000, "silu_gate", 100, 128),    # gated: 12 in a ring of four
+    (2, 700, 328, 9000, "silu_gate", None, 128),
+    (3, 2000, 584, 4000, "silu", None, 256),       # wide
+    (2, 1500, 456, 5000, "gelu_tanh", 80, 256),
+])
+def test_grouped_many_tiles(gpu, ops, X, M, K, N, act, gather, bn):
+    """More tiles than SMs, so that a CTA runs several: the accumulators take
+    turns, the ring wraps within and across tiles, an epilogue overlaps the next
+    tile's products."""
+    from tests.test_moe_gpu import assert_within, run_grouped
+    tile, splits, most, kb = grouped_plan(X, M, K, N, act == "silu_gate")
+    real = (M // tile) * -(-N // 128)
+    assert (tile, splits) == (bn, 1) and max(real, X // 2 * -(-N // 128)) > 1.2 * SMS and kb > 4
+    rng = np.random.default_rng(M + K)
+    for dt in ("bf16", "f16"):
+        assert_within(*run_grouped(ops, rng, dt, X, M, K, N, act, True, gather), f"{X} {M} {K} {N} {act} {dt}")
+    assert device_error(0) == 0
+
+
+def test_grouped_long_group_in_narrow_tiles(gpu, ops):
+    """Every row in one of many groups: the mean says narrow tiles, the group
+    is cut into many of them."""
+    from tests.test_moe_gpu import assert_within, run_grouped
+    rng = np.random.default_rng(31)
+    for act, N in (("none", 1200), ("silu_gate", 600)):
+        offsets = np.zeros(65, np.int32)
+        offsets[38:] = 997
+        assert_within(*run_grouped(ops, rng, "bf16", 64, 997, 520, N, act, True, 50, offsets=offsets))
+    assert device_error(0) == 0
+
+
+_FIRST_IN_CAPTURE = """
+import ctypes as C, numpy as np, sys
+from scaffolding_b200 import _cuda_ops as ops, engine as E
+bf = E.bfloat16
+rng = np.random.default_rng(0)
+N, K, M = 16392, 4064, {M}
+q = rng.integers(0, 16, (N, K)).astype(np.uint8)
+s = np.full((N, 32), 2.0 ** -8, np.float32).astype(bf)
+w4 = ops.W4Weight.from_arrays(q, s, None, 128, 0)
+x = rng.integers(-3, 4, (M, K)).astype(np.float32)
+gx = ops.gputensor_from_numpy(x.astype(bf), 0)
+out = ops._alloc((M, N), np.float32, 0)
+st = ops.CudaStream(0)
+E.set_stream(0, st.cuda_stream)
+E.check(E.lib.sf_graph_begin(C.c_void_p(st.cuda_stream)), "begin")
+ops.dev_linear_w4(gx, w4, out=out)
+exe = C.c_void_p()
+E.check(E.lib.sf_graph_end(C.c_void_p(st.cuda_stream), C.byref(exe)), "end")
+for _ in range(2):
+    E.check(E.lib.sf_graph_launch(exe, C.c_void_p(st.cuda_stream)), "launch")
+st.synchronize()
+y = ops.gputensor_to_numpy(out)
+# whole numbers below 2^24 over a power of two: every sum is exact
+ref = (x.astype(np.float64) @ (q.astype(np.float64) - 8).T) / 256
+assert np.array_equal(y, ref), np.abs(y - ref).max()
+assert E.device_error_status(0) == 0
+print("exact")
+"""
+
+
+@pytest.mark.parametrize("M", [1, 16, 40])
+def test_first_call_of_a_process_in_a_capture(gpu, M):
+    """The first 4-bit linear of a process is captured: the opt-in to shared
+    memory and the question of how many clusters fit come inside the capture."""
+    import subprocess
+    import sys
+
+    from tests.conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", _FIRST_IN_CAPTURE.format(M=M)], cwd=ROOT, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "exact" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dt,sdt", [("f32", "bf16"), ("f32", "f16"), ("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("N,K,group", [(33, 300, 32), (64, 512, 128), (7, 200, 64)])
+def test_quantised_values(gpu, ops, dt, sdt, zeros, N, K, group):
+    """Scale, zero point and every 4-bit value of the stored weight: those of
+    the definition, from the stored scale on.  Quotients are divided in fp32 on
+    both sides; where one lies within 2^-20 of a tie either neighbour is right
+    (fp32 rounding of a quotient below 16: 2^-21)."""
+    rng = np.random.default_rng(N + K)
+    w = rng.standard_normal((N, K), dtype=np.float32)
+    w[0, :group] = 0
+    w[1, :group] = np.abs(w[1, :group])   # a range without negative values
+    w[2, :group] = -np.abs(w[2, :group])
+    gw, w = to_device(ops, w, dt)
+    w4 = ops.dev_quantize_w4(gw, group, zeros, np_dtype(sdt))
+    words = ops.gputensor_to_numpy(w4.packed)
+    q = np.zeros((N, words.shape[1] * 8), np.int64)
+    for t in range(4):
+        for j in range(4):
+            for i, c in enumerate((0, 2, 4, 6, 1, 3, 5, 7)):
+                q[:, 32 * j + 8 * t + c::128] = (words[:, 4 * t + j::16] >> np.uint32(4 * i)) & 15
+    s = to_host32(ops, w4.scales).astype(np.float64).T
+    z = to_host32(ops, w4.zeros).T if zeros else np.full(s.shape, 8.0)
+    for g in range(s.shape[1]):
+        cols = slice(g * group, min(K, (g + 1) * group))
+        v = w[:, cols].astype(np.float64)
+        lo, hi = np.minimum(v.min(1), 0), np.maximum(v.max(1), 0)
+        exact = (hi - lo) / 15 if zeros else np.maximum(hi, -lo) / 7
+        # one rounding of the difference, one of the quotient, one to the scale's type
+        step = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11}[sdt]
+        assert (np.abs(s[:, g] - exact) <= (step + 2.0 ** -22) * exact + 2.0 ** -25).all()
+        live = s[:, g] > 0
+        some = np.where(live, s[:, g], 1.0)
+        if zeros:
+            ideal = np.where(live, -lo / some, 0.0)
+            clear = np.abs(ideal - np.floor(ideal) - 0.5) > 2.0 ** -20
+            assert np.array_equal(z[clear, g], np.clip(np.rint(ideal), 0, 15)[clear])
+            assert (np.abs(z[:, g] - ideal) <= 0.5 + 2.0 ** -20).all() and (z[:, g] == np.rint(z[:, g])).all()
+        ideal = np.where(live[:, None], v / some[:, None], 0.0)
+        clear = np.abs(ideal - np.floor(ideal) - 0.5) > 2.0 ** -20
+        want = np.clip(np.rint(ideal) + z[:, g, None], 0, 15)
+        assert np.array_equal(q[:, cols][clear], want[clear])
+        assert (np.abs(q[:, cols] - want) <= 1).all()
+        assert (q[~live][:, cols] == z[~live, g, None]).all()
