@@ -49,6 +49,13 @@ static std::vector<DeviceInfo> g_devs;
 int32_t current_device_info(DeviceInfo** out, int* device) {
   int dev = 0;
   SF_CUDA_TRY(cudaGetDevice(&dev));
+  // A host thread has no context before its first call that needs one, and the
+  // driver's tensor-map encoder, which a launch comes to first, does not make it.
+  static thread_local int bound = -1;
+  if (bound != dev) {
+    SF_CUDA_TRY(cudaSetDevice(dev));
+    bound = dev;
+  }
   std::lock_guard<std::mutex> lk(g_dev_mu);
   if (g_devs.empty()) {
     int n = 0;

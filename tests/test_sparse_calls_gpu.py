@@ -393,3 +393,35 @@ def test_quantised_values(gpu, ops, dt, sdt, zeros, N, K, group):
         assert np.array_equal(q[:, cols][clear], want[clear])
         assert (np.abs(q[:, cols] - want) <= 1).all()
         assert (q[~live][:, cols] == z[~live, g, None]).all()
+
+
+def test_first_call_of_a_thread(gpu, ops):
+    """A host thread whose first use of the device is a launch into kept
+    buffers: the driver has no context on it yet."""
+    from scaffolding_b200._lib import check, lib
+    rng = np.random.default_rng(3)
+    x = {M: to_device(ops, rng.standard_normal((M, 256), dtype=np.float32), "bf16")[0] for M in (4, 40)}
+    gw, _ = to_device(ops, rng.standard_normal((128, 256), dtype=np.float32), "bf16")
+    g3 = ops.dev_reshape(gw, (1, 128, 256))
+    w4 = ops.dev_quantize_w4(gw, 64)
+    sw, _ = to_device(ops, rng.standard_normal((16384, 4096), dtype=np.float32), "bf16")
+    sx, _ = to_device(ops, rng.standard_normal((2, 4096), dtype=np.float32), "bf16")
+    big = ops.dev_quantize_w4(sw, 128)
+    off = ops.gputensor_from_numpy(np.array([0, 40], np.int32))
+
+    def noalloc(out):
+        check(lib.sf_linear_skinny_noalloc(40, 128, 256, x[40].ptr, 256, gw.ptr, 256, None, 0, out.ptr, 128, 2, 2,
+                                           0, None), "sf_linear_skinny_noalloc")
+
+    calls = [((40, 128), lambda out: ops.dev_grouped_linear(x[40], g3, off, out=out)),
+             ((40, 128), lambda out: ops.dev_linear_w4(x[40], w4, out=out)),
+             ((4, 128), lambda out: ops.dev_linear_w4(x[4], w4, out=out)),
+             ((2, 16384), lambda out: ops.dev_linear_w4(sx, big, out=out)),
+             ((40, 128), lambda out: ops.dev_linear_forward(x[40], gw, out=out)),
+             ((40, 128), noalloc)]
+    for shape, call in calls:
+        want, got = (ops.gputensor_from_numpy(np.full(shape, v).astype(np_dtype("bf16"))) for v in (1, 2))
+        call(want)
+        _in_threads(lambda: call(got))
+        assert np.array_equal(to_host32(ops, got), to_host32(ops, want))
+    assert device_error(0) == 0
