@@ -1016,8 +1016,11 @@ class CudaStream:
     def __del__(self):
         try:
             if self._stream:
-                lib.sf_stream_destroy(C.c_void_p(self._stream))
-                self._stream = None
+                try:
+                    E.release_stream(self._stream)
+                finally:
+                    lib.sf_stream_destroy(C.c_void_p(self._stream))
+                    self._stream = None
         except Exception:
             pass
 

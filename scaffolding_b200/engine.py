@@ -247,6 +247,17 @@ def workspace(dev: int, stream: int | None, nbytes: int, use: str = "sums") -> D
         return buf
 
 
+def release_stream(stream: int) -> None:
+    """Return the workspaces of a stream that is about to be destroyed: another
+    may come to have its address.  Those of captures stay."""
+    with workspace_lock:
+        keys = [key for key in _workspaces if key[1] == stream]
+        if keys:
+            stream_sync(stream)
+        for key in keys:
+            _workspaces.pop(key).free()
+
+
 def release_workspaces(captured: bool = False) -> None:
     """Return the workspaces to the pool once nothing queued uses them; with
     ``captured`` those of captures too, whose graphs must be gone."""

@@ -386,3 +386,23 @@ def test_route_leaves_room_for_its_index_arithmetic():
     blocks = sz.value // (64 * 4)
     chunk = -(-most // 512)
     assert blocks == -(-most // chunk) and blocks * chunk + 16 * 4 < 1 << 31
+
+
+def test_a_streams_workspaces_go_with_it(ops, engine):
+    """A destroyed stream's workspaces return to the pool, waited for: another
+    stream may come to have its address."""
+    from scaffolding_b200 import engine as E
+    engine.patch("sf_stream_create", lambda dev, nb, out: engine._set(out, 4242))
+    engine.patch("sf_stream_destroy", lambda s: engine.note("destroy", getattr(s, "value", s)))
+    s = ops.CudaStream(0)
+    mine, legacy = E.workspace(0, s.cuda_stream, 100).ptr, E.workspace(0, None, 100).ptr
+    more = E.workspace(0, s.cuda_stream, 100, "weight").ptr
+    engine.capture_id[4242] = 9
+    graphs = E.workspace(0, s.cuda_stream, 100).ptr
+    engine.capture_id[4242] = 0
+    del s
+    calls = [(c, getattr(what, "value", what)) for c, _, what in engine.log]
+    freed = [p for c, p in calls if c == "free"]
+    assert sorted(freed) == sorted([mine, more]) and graphs not in freed and legacy not in freed
+    assert calls.index(("sync", 4242)) < calls.index(("free", mine)) and ("destroy", 4242) in calls
+    assert list(E._workspaces) == [(0, 0, "sums")]
