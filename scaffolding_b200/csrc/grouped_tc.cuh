@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(Cfg::THREADS + 32 * Cfg::GATHER_WARPS, 1)
         // The partial sums take the ring's place: every copy into it was
         // waited for and every MMA that read it has completed.
         if (kb0 >= kb1) break;
-        if (!mbar_wait(&tfull_bar[0], 0, p.err, kDevTimeoutEpilogue, abortp)) break;
+        // One outcome for the warp, here and below: TMEM loads of all its lanes follow.
+        if (!__all_sync(0xffffffffu, mbar_wait(&tfull_bar[0], 0, p.err, kDevTimeoutEpilogue, abortp))) break;
         tc_fence_after();
         float* part = reinterpret_cast<float*>(smem) + quad * 32 + lane;
         for (int c = half * CH; c < t.rows; c += 2 * CH)
@@ -430,7 +431,8 @@ __global__ void __launch_bounds__(Cfg::THREADS + 32 * Cfg::GATHER_WARPS, 1)
         bias0 = load_as_f32(p.bias, t.g * p.bias_stride + n, p.bias_dtype);
         if constexpr (Cfg::GATE) bias1 = load_as_f32(p.bias, t.g * p.bias_stride + p.N + n, p.bias_dtype);
       }
-      if (!mbar_wait(&tfull_bar[acc], acc_phase, p.err, kDevTimeoutEpilogue, abortp)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull_bar[acc], acc_phase, p.err, kDevTimeoutEpilogue, abortp)))
+        break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
                              static_cast<uint32_t>(acc * Cfg::ACC_COLS);
