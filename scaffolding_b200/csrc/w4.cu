@@ -488,7 +488,8 @@ int32_t run_w4(const W4Args& a, cudaStream_t s) {
 //   with zeros: s = (max - min) / 15 rounded likewise, z = rint(-min / s),
 //               q = rint(w / s) + z; max and min taken with 0 included, so
 //               that z lies in 0..15 and a weight of 0 is kept exactly
-// q clamped to 0..15; s = 0 (an all-zero group) stores q = z.
+// q clamped to 0..15; s = 0 (an all-zero group) stores q = z.  A group with a
+// NaN or an infinity, which no q stands for, has a scale of NaN.
 __global__ void __launch_bounds__(128) w4_quantize_kernel(int N, int K, const void* W, int w_dtype,
                                                           int64_t ldw, int group, uint8_t* q8,
                                                           int64_t ld8, void* scales, void* zeros,
@@ -499,12 +500,15 @@ __global__ void __launch_bounds__(128) w4_quantize_kernel(int N, int K, const vo
   const int n = static_cast<int>(i / groups), g = static_cast<int>(i - n * groups);
   const int k0 = g * group, k1 = min(K, k0 + group);
   float lo = 0.0f, hi = 0.0f;
+  bool finite = true;
   for (int k = k0; k < k1; ++k) {
     const float w = load_as_f32(W, n * ldw + k, w_dtype);
+    finite = finite && fabsf(w) < INFINITY;
     lo = fminf(lo, w);
     hi = fmaxf(hi, w);
   }
-  store_from_f32(scales, g * lds + n, s_dtype, zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f);
+  store_from_f32(scales, g * lds + n, s_dtype,
+                 !finite ? NAN : zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f);
   const float s = load_as_f32(scales, g * lds + n, s_dtype);
   float z = 8.0f;
   if (zeros) {

@@ -425,3 +425,25 @@ def test_first_call_of_a_thread(gpu, ops):
         _in_threads(lambda: call(got))
         assert np.array_equal(to_host32(ops, got), to_host32(ops, want))
     assert device_error(0) == 0
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_quantised_non_finite_weights(gpu, ops, zeros, bad):
+    """A NaN or infinite weight makes its group NaN, and the outputs of its row,
+    as it does in a plain linear; it is not turned into a number."""
+    rng = np.random.default_rng(6)
+    w = rng.standard_normal((20, 256), dtype=np.float32)
+    w[3, 70] = bad
+    w[9, 128:192] = bad
+    gw, w = to_device(ops, w, "bf16")
+    w4 = ops.dev_quantize_w4(gw, 64, zeros)
+    back = to_host32(ops, ops.dev_dequantize_w4(w4))
+    nan = np.zeros(w.shape, bool)
+    nan[3, 64:128] = nan[9, 128:192] = True
+    assert np.array_equal(np.isnan(back), nan) and np.isfinite(back[~nan]).all()
+    for M in (1, 40):
+        gx, _ = to_device(ops, rng.standard_normal((M, 256), dtype=np.float32), "bf16")
+        y = to_host32(ops, ops.dev_linear_w4(gx, w4))
+        assert np.array_equal(np.isnan(y), np.broadcast_to(nan.any(1), y.shape))
+    assert device_error(0) == 0
