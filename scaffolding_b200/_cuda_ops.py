@@ -622,8 +622,11 @@ _W4_MAX_ROWS = 64  # rows of x that sf_linear_w4 takes
 def pack_w4(q: np.ndarray) -> np.ndarray:
     """Host ``[N, K]`` values 0..15 to ``[N, 16 * ceil(K / 128)]`` uint32
     words in the order ``sf_linear_w4`` documents; columns past K hold 0."""
-    if q.ndim != 2 or (q.size and (q.min() < 0 or q.max() > 15)):
-        raise ValueError("4-bit values are a 2-d array of 0..15")
+    if q.dtype.kind == "V":  # ml_dtypes' small types
+        q = q.astype(np.float32)
+    if q.ndim != 2 or q.dtype.kind not in "uibf" or (q.size and not (
+            q.min() >= 0 and q.max() <= 15 and (q.dtype.kind != "f" or (q == np.rint(q)).all()))):
+        raise ValueError("4-bit values are a 2-d array of whole numbers 0..15")
     n, k = q.shape
     blocks = -(-k // 128)
     padded = np.zeros((n, blocks * 128), np.uint32)

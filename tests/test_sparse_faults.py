@@ -406,3 +406,14 @@ def test_a_streams_workspaces_go_with_it(ops, engine):
     assert sorted(freed) == sorted([mine, more]) and graphs not in freed and legacy not in freed
     assert calls.index(("sync", 4242)) < calls.index(("free", mine)) and ("destroy", 4242) in calls
     assert list(E._workspaces) == [(0, 0, "sums")]
+
+
+def test_packing_refuses_what_is_no_whole_number(ops):
+    """Values that 4 bits do not hold are not cut to ones that they do."""
+    for bad in ([[1.5]], [[np.nan]], [[np.inf]], [[16.0]], [[-1]], [["3"]], [[2 + 0j]]):
+        with pytest.raises(ValueError, match="0..15"):
+            ops.pack_w4(np.array(bad))
+    for dtype in (np.uint8, np.int64, np.float32, np.float16, ops.bfloat16, bool):
+        q = np.array([[1, 0] * 70], dtype)
+        assert np.array_equal(ops.pack_w4(q), ops.pack_w4(q.astype(np.uint8)))
+    assert ops.pack_w4(np.zeros((0, 5), np.uint8)).shape == (0, 16)
