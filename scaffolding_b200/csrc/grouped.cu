@@ -73,9 +73,10 @@ bool gather_pays(int64_t groups, int64_t M, int64_t N) {
 int64_t gathered_ld(int64_t K) { return (K + 7) / 8 * 8; }
 
 // out[i, :] = A[rows[i], :], zeros for an index outside A; a warp per row, 16
-// bytes per lane and step.  What lies past K in a row's last vector is copied
-// along (it is inside the row of A, which starts on 16-byte boundaries) and
-// not used.
+// bytes per lane and step (plain loads: the rows may have been written while
+// this grid, launched early, already ran, which read-only loads exclude).  What
+// lies past K in a row's last vector is copied along (it is inside the row of A,
+// which starts on 16-byte boundaries) and not used.
 __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* A, int64_t ld_vec, int64_t a_rows,
                                                           const int* rows, int M, int vecs, uint4* out) {
   pdl_launch_dependents();
@@ -90,7 +91,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* A, int64_
       uint4 u[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        u[j] = in && v + 32 * j < vecs ? __ldg(src + v + 32 * j) : make_uint4(0, 0, 0, 0);
+        u[j] = in && v + 32 * j < vecs ? src[v + 32 * j] : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (v + 32 * j < vecs) dst[v + 32 * j] = u[j];

@@ -80,10 +80,11 @@ __device__ __forceinline__ void unpack_word(uint32_t w, uint2 z, uint32_t (&p)[4
 
 // A scale or zero point ahead of its use.  A register of its own for each, and
 // no branch or select on the value: either would make the load be waited for
-// where it is issued (250 cycles each, measured).
+// where it is issued (250 cycles each, measured).  Not a read-only load: the grid
+// may have been launched before what it reads was written.
 __device__ __forceinline__ uint32_t load_ahead(const uint16_t* p) {
   uint32_t v;
-  asm volatile("{\n\t.reg .u16 t;\n\tld.global.nc.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(v) : "l"(p));
+  asm volatile("{\n\t.reg .u16 t;\n\tld.global.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(v) : "l"(p));
   return v;
 }
 
