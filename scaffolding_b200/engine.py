@@ -240,7 +240,8 @@ def workspace(dev: int, stream: int | None, nbytes: int, use: str = "sums") -> D
         buf = _workspaces.get(key)
         if buf is None or buf.nbytes < nbytes:
             if buf is not None:
-                stream_sync(stream)
+                with on_device(dev):
+                    stream_sync(stream)
                 buf.free()
             buf = DeviceBuffer.alloc(nbytes, dev)
             _workspaces[key] = buf
@@ -253,7 +254,8 @@ def release_stream(stream: int) -> None:
     with workspace_lock:
         keys = [key for key in _workspaces if key[1] == stream]
         if keys:
-            stream_sync(stream)
+            with on_device(keys[0][0]):
+                stream_sync(stream)
         for key in keys:
             _workspaces.pop(key).free()
 

@@ -417,3 +417,21 @@ def test_packing_refuses_what_is_no_whole_number(ops):
         q = np.array([[1, 0] * 70], dtype)
         assert np.array_equal(ops.pack_w4(q), ops.pack_w4(q.astype(np.uint8)))
     assert ops.pack_w4(np.zeros((0, 5), np.uint8)).shape == (0, 16)
+
+
+def test_outgrown_workspace_waits_on_its_device(engine):
+    """The legacy stream that is waited for is that of the workspace's device,
+    whichever device is current."""
+    from scaffolding_b200 import engine as E
+    current = [0]
+
+    def set_device(dev):
+        current[0] = dev
+        return 0
+
+    engine.patch("sf_get_device", lambda out: engine._set(out, current[0]))
+    engine.patch("sf_set_device", set_device)
+    engine.patch("sf_stream_synchronize", lambda s: engine.note("sync on", current[0]))
+    E.workspace(1, None, 100)
+    E.workspace(1, None, 9000)
+    assert [what for c, _, what in engine.log if c == "sync on"] == [1] and current == [0]
