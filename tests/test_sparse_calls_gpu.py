@@ -447,3 +447,51 @@ def test_quantised_non_finite_weights(gpu, ops, zeros, bad):
         y = to_host32(ops, ops.dev_linear_w4(gx, w4))
         assert np.array_equal(np.isnan(y), np.broadcast_to(nan.any(1), y.shape))
     assert device_error(0) == 0
+
+
+@pytest.mark.parametrize("act", ["none", "silu_gate"])
+def test_captured_gather_of_a_long_batch(gpu, ops, act):
+    """A captured batch gathers its rows as it reads them, a direct one copies
+    them first: the same bits."""
+    rng = np.random.default_rng(41)
+    X, M, K, N, T = 5, 2600, 264, 1030, 700
+    wide = 2 * N if act == "silu_gate" else N
+    gx, _ = to_device(ops, rng.standard_normal((T, K), dtype=np.float32), "bf16")
+    gw, _ = to_device(ops, rng.standard_normal((X, wide, K), dtype=np.float32) / np.float32(16), "bf16")
+    rows = ops.gputensor_from_numpy(rng.integers(-1, T + 1, M).astype(np.int32))
+    off = ops.gputensor_from_numpy(np.array([0, 700, 700, 1500, 2590, M], np.int32))
+    want = to_host32(ops, ops.dev_grouped_linear(gx, gw, off, activation=act, rows=rows))
+    out = ops._alloc((M, N), np_dtype("bf16"), 0)
+    with Capture(ops) as g:
+        ops.dev_grouped_linear(gx, gw, off, activation=act, rows=rows, out=out)
+    for _ in range(2):
+        g.launch()
+    g.stream.synchronize()
+    assert np.array_equal(to_host32(ops, out), want)
+    g.destroy()
+    assert device_error(0) == 0
+
+
+@pytest.mark.parametrize("M", [300, 70000])
+def test_grouped_most_groups(gpu, ops, M):
+    """4096 groups, most of them empty or of a few rows, in narrow and in wide
+    tiles; their bounds take the most shared memory there can be."""
+    from tests.test_moe_gpu import assert_within, run_grouped
+    rng = np.random.default_rng(M)
+    counts = np.bincount(np.minimum(rng.geometric(1 / 300, M) - 1, 4095), minlength=4096)
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    for act in ("none", "silu_gate"):
+        for gather in (None, 90):
+            assert_within(*run_grouped(ops, rng, "bf16", 4096, M, 72, 20, act, True, gather, offsets=offsets))
+    assert device_error(0) == 0
+
+
+def test_combine_without_rows(gpu, ops):
+    """No expert rows at all: the residual alone, or zeros."""
+    rng = np.random.default_rng(0)
+    gr, res = to_device(ops, rng.standard_normal((6, 40), dtype=np.float32), "bf16")
+    y = ops._alloc((0, 40), np_dtype("bf16"), 0)
+    s = ops.gputensor_from_numpy(np.array([[0, -1]] * 6, np.int32))
+    w = ops.gputensor_from_numpy(np.ones((6, 2), np.float32))
+    assert np.array_equal(to_host32(ops, ops.dev_moe_combine(y, s, w, gr)), res)
+    assert not to_host32(ops, ops.dev_moe_combine(y, s, w)).any()
