@@ -557,7 +557,9 @@ bool known_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
 int32_t check_w4(int64_t N, int64_t K, const void* packed, int64_t ldp, const void* scales,
                  int64_t lds, int32_t group) {
   if (N < 0 || K < 0) return fail(SF_ERR_INVALID_ARGUMENT, "negative dimension");
-  if (N > INT32_MAX || K > INT32_MAX - 127) return fail(SF_ERR_UNSUPPORTED, "dimension exceeds 2^31-1");
+  // Row and column numbers are rounded up to tiles in 32 bits.
+  constexpr int64_t kMost = INT32_MAX - 4096;
+  if (N > kMost || K > kMost) return fail(SF_ERR_UNSUPPORTED, "dimension exceeds 2^31-4097");
   if (group != 32 && group != 64 && group != 128)
     return fail(SF_ERR_UNSUPPORTED, "group of %d columns (32, 64 or 128)", group);
   if (N == 0 || K == 0) return SF_OK;

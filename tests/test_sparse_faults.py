@@ -435,3 +435,20 @@ def test_outgrown_workspace_waits_on_its_device(engine):
     E.workspace(1, None, 100)
     E.workspace(1, None, 9000)
     assert [what for c, _, what in engine.log if c == "sync on"] == [1] and current == [0]
+
+
+def test_w4_leaves_room_for_its_index_arithmetic():
+    """Row and column numbers rounded up to a tile are 32-bit numbers too (the
+    addresses are never read: the refusals, and an empty x, come first)."""
+    import ctypes as C
+
+    from scaffolding_b200._lib import SF_ERR_UNSUPPORTED as NO, lib
+    p = C.c_void_p(4096)
+    most = (1 << 31) - 4097
+
+    def call(N, K):
+        return lib.sf_linear_w4(0, N, K, p, K, p, -(-K // 128) * 16, p, None, N, 128, None, 0, p, N, 2, 2, 0, None)
+
+    assert call(most, 128) == 0 and call(8, most) == 0
+    for N, K in ((most + 1, 128), ((1 << 31) - 1, 128), (8, most + 1), (8, (1 << 31) - 128)):
+        assert call(N, K) == NO
