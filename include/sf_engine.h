@@ -172,8 +172,8 @@ int32_t sf_linear_skinny_noalloc(int64_t M, int64_t N, int64_t K,
  *   groups b_stride apart (0: one weight for all); bias likewise, bias_stride
  *   apart, or NULL.  C shares no memory with the inputs.
  * 16-bit operands whose rows start on 16-byte boundaries run on the tensor
- * cores; fp32 and other layouts on the FMA pipe (IEEE fp32).  At most 4096
- * groups.  The workspace is optional: with
+ * cores; fp32 and other layouts on the FMA pipe (IEEE fp32, whose grid holds M /
+ * 64 + min(groups, M) <= 65535).  At most 4096 groups.  The workspace is optional: with
  * sf_gemm_grouped_workspace_size() bytes of it (16-byte aligned), a call with
  * many rows to gather copies them there first (one launch more), without it
  * they are gathered as they are read; the result is the same, bit for bit.
@@ -198,10 +198,10 @@ int32_t sf_gemm_grouped_workspace_size(int64_t groups, int64_t M, int64_t N, int
  *   slot p of offsets[e] <= p < offsets[e + 1] holds token rows[p], by rising
  *   token; slots[t][j] is the slot of choice j of token t.
  * expert_ids, weights and slots are [tokens][top_k], rows [tokens * top_k],
- * offsets [experts + 1].  At most 1024 experts, top_k 32 and tokens * top_k
- * of 2^31 - 2^23 - 1.  The same
- * inputs give the same bits.  The workspace (0 bytes for few tokens) is free
- * again when the call's kernels are done.  No counterpart in the reference. */
+ * offsets [experts + 1]; none of them shares memory with the logits.  At most
+ * 1024 experts, top_k 32 and tokens * top_k of 2^31 - 2^23 - 1.  The same inputs
+ * give the same bits.  The workspace (0 bytes for few tokens) is free again when
+ * the call's kernels are done.  No counterpart in the reference. */
 int32_t sf_moe_route_workspace_size(int64_t tokens, int64_t experts, int32_t top_k, size_t* bytes);
 int32_t sf_moe_route(int64_t tokens, int64_t experts, int32_t top_k, const void* logits,
                      int32_t dtype, int64_t ld, int32_t renormalize, int32_t* expert_ids,
@@ -210,8 +210,9 @@ int32_t sf_moe_route(int64_t tokens, int64_t experts, int32_t top_k, const void*
 
 /* out[t, :] = residual[t, :] + sum_j weights[t][j] * y[slots[t][j], :] in
  * fp32, rounded once (residual may be NULL; y, residual and out share dtype).
- * A slot outside 0..y_rows-1 adds nothing.  out may be residual's memory, not
- * y's.  No counterpart in the reference. */
+ * A slot outside 0..y_rows-1 adds nothing.  out may be residual's memory, with
+ * its leading dimension, and shares none with the other inputs.  No
+ * counterpart in the reference. */
 int32_t sf_moe_combine(int64_t tokens, int64_t cols, int32_t top_k, const void* y, int64_t y_rows,
                        int64_t ldy, int32_t dtype, const int32_t* slots, const float* weights,
                        const void* residual, int64_t ldr, void* out, int64_t ldo, void* stream);
@@ -228,7 +229,7 @@ int32_t sf_moe_combine(int64_t tokens, int64_t cols, int32_t top_k, const void* 
  * ceil(K / 128) words (16-byte aligned, ldp a multiple of 4): nibble i (from
  * the low end) of word 4 t + w of 128-column block b holds column
  *   128 b + 32 w + 8 t + {0, 2, 4, 6, 1, 3, 5, 7}[i]
- * (columns past K are ignored).  Sums in fp32.  Beside the skinny linears of
+ * (columns past K are ignored).  N and K up to 2^31 - 4097.  Sums in fp32.  Beside the skinny linears of
  * sf_gemm; no counterpart in the reference. */
 int32_t sf_linear_w4(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
                      const uint32_t* packed, int64_t ldp, const void* scales, const void* zeros,
@@ -239,7 +240,8 @@ int32_t sf_linear_w4(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx
 /* Quantises W [N,K] into that form.  zeros NULL: scale = max|w| / 7,
  * q = rint(w / scale) + 8; else scale = (max - min) / 15 (0 counted in),
  * zero = rint(-min / scale), q = rint(w / scale) + zero; the scale is rounded
- * to scale_dtype before q is formed.  sf_dequantize_w4 writes W back in
+ * to scale_dtype before q is formed.  A group with a NaN or an infinity has a
+ * scale of NaN.  sf_dequantize_w4 writes W back in
  * w_dtype, one rounding, for products with more rows. */
 int32_t sf_quantize_w4(int64_t N, int64_t K, const void* W, int32_t w_dtype, int64_t ldw,
                        int32_t group, uint32_t* packed, int64_t ldp, void* scales, void* zeros,
@@ -406,7 +408,8 @@ int32_t sf_event_elapsed_ms(void* start, void* end, float* ms);
 /* CUDA graphs: capture the launches issued on `stream` between begin and end
  * (relaxed capture mode) into an executable graph, then replay it.  For
  * launch-bound sequences such as skinny-M GEMMs.  New (the reference has no
- * graph support).  Workspaces must already be sized before capture. */
+ * graph support).  A workspace given to a captured call belongs to the graph:
+ * another call that uses it between replays, or frees it, changes its results. */
 int32_t sf_graph_begin(void* stream);
 int32_t sf_graph_end(void* stream, void** exec);
 int32_t sf_graph_launch(void* exec, void* stream);

@@ -29,6 +29,11 @@ struct DeviceInfo {
   int* err_word = nullptr;  // device-side error word (cudaMalloc'd once per device)
 };
 
+// Makes the context of `device`, the current one, current on this host thread if
+// none is: the driver's tensor-map encoder needs one, and a thread that has not
+// used the device has none.  A context of the caller's own stays.
+int32_t bind_context(int device);
+
 // Lazily initialised per-device facts for the CURRENT device.
 int32_t current_device_info(DeviceInfo** out, int* device);
 

@@ -77,14 +77,10 @@ int32_t set_attrs_fmt() {
 
 // Once per device, with `device` current.
 int32_t setup(int device, NoAllocDevice** out) {
-  // The tensor-map encoder needs the device's context on this host thread.
-  static thread_local int bound = -1;
-  if (bound != device) {
-    SF_CUDA_TRY(cudaSetDevice(device));
-    bound = device;
-  }
   std::lock_guard<std::mutex> lk(g_mu);
   if (device < 0 || device >= 64) return fail(SF_ERR_INVALID_ARGUMENT, "device %d out of range", device);
+  const int32_t bound = bind_context(device);
+  if (bound != SF_OK) return bound;
   NoAllocDevice& d = g_dev[device];
   if (!d.ready) {
     void* p = nullptr;

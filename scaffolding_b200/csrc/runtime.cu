@@ -9,6 +9,7 @@
 // called with the GIL released, and its cap defaults to 32 GiB instead of
 // 2 GB because a B200 holds 180 GB and the attention score buffers of the
 // DiT workload alone are several GB.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -46,16 +47,31 @@ int32_t cuda_status(cudaError_t e, const char* what) {
 static std::mutex g_dev_mu;
 static std::vector<DeviceInfo> g_devs;
 
+int32_t bind_context(int device) {
+  static thread_local bool bound = false;
+  if (bound) return SF_OK;
+  using GetCurrentFn = CUresult (*)(CUcontext*);
+  static const GetCurrentFn get_current = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      p = nullptr;
+    }
+    return reinterpret_cast<GetCurrentFn>(p);
+  }();
+  CUcontext context = nullptr;
+  if (!get_current || get_current(&context) != CUDA_SUCCESS || !context) SF_CUDA_TRY(cudaSetDevice(device));
+  bound = true;
+  return SF_OK;
+}
+
 int32_t current_device_info(DeviceInfo** out, int* device) {
   int dev = 0;
   SF_CUDA_TRY(cudaGetDevice(&dev));
-  // A host thread has no context before its first call that needs one, and the
-  // driver's tensor-map encoder, which a launch comes to first, does not make it.
-  static thread_local int bound = -1;
-  if (bound != dev) {
-    SF_CUDA_TRY(cudaSetDevice(dev));
-    bound = dev;
-  }
+  const int32_t st = bind_context(dev);
+  if (st != SF_OK) return st;
   std::lock_guard<std::mutex> lk(g_dev_mu);
   if (g_devs.empty()) {
     int n = 0;
