@@ -569,6 +569,9 @@ extern "C" int32_t sf_moe_combine(int64_t tokens, int64_t cols, int32_t top_k, c
     return fail(SF_ERR_INVALID_ARGUMENT, "null pointer");
   if (ldy < cols || ldo < cols || (residual && ldr < cols))
     return fail(SF_ERR_INVALID_ARGUMENT, "leading dimension < cols");
+  if (residual == out && ldr != ldo && tokens > 1)
+    return fail(SF_ERR_INVALID_ARGUMENT, "in place needs one leading dimension (%lld, %lld)", (long long)ldr,
+                (long long)ldo);
   DeviceInfo* dev = nullptr;
   const int32_t st = current_device_info(&dev, nullptr);
   if (st != SF_OK) return st;

@@ -452,3 +452,17 @@ def test_w4_leaves_room_for_its_index_arithmetic():
     assert call(most, 128) == 0 and call(8, most) == 0
     for N, K in ((most + 1, 128), ((1 << 31) - 1, 128), (8, most + 1), (8, (1 << 31) - 128)):
         assert call(N, K) == NO
+
+
+def test_combine_into_a_residual_of_another_stride():
+    """In place means row on row: with other strides one token's result would
+    be written over another's residual."""
+    import ctypes as C
+
+    from scaffolding_b200._lib import SF_ERR_INVALID_ARGUMENT as BAD, lib
+    p, r = C.c_void_p(4096), C.c_void_p(1 << 20)
+
+    def call(tokens, ldr, ldo):
+        return lib.sf_moe_combine(tokens, 8, 2, p, 8, 8, 2, p, p, r, ldr, r, ldo, None)
+
+    assert call(2, 8, 16) == BAD and call(5, 24, 8) == BAD
