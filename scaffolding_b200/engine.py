@@ -242,6 +242,7 @@ def workspace(dev: int, stream: int | None, nbytes: int, use: str = "sums") -> D
             if buf is not None:
                 with on_device(dev):
                     stream_sync(stream)
+                del _workspaces[key]
                 buf.free()
             buf = DeviceBuffer.alloc(nbytes, dev)
             _workspaces[key] = buf

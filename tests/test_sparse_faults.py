@@ -466,3 +466,16 @@ def test_combine_into_a_residual_of_another_stride():
         return lib.sf_moe_combine(tokens, 8, 2, p, 8, 8, 2, p, p, r, ldr, r, ldo, None)
 
     assert call(2, 8, 16) == BAD and call(5, 24, 8) == BAD
+
+
+def test_workspace_after_running_out_of_memory(engine):
+    """A growth that fails leaves no freed buffer behind for smaller calls."""
+    from scaffolding_b200 import engine as E
+    from scaffolding_b200._lib import EngineError
+    E.workspace(0, None, 100)
+    malloc = engine._malloc
+    engine.patch("sf_malloc", lambda dev, n, out: -4 if n > 1000 else malloc(dev, n, out))
+    with pytest.raises(EngineError):
+        E.workspace(0, None, 5000)
+    buf = E.workspace(0, None, 100)
+    assert buf.ptr and buf.nbytes >= 100
