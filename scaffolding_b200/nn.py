@@ -189,6 +189,7 @@ class MoE:
             self.to(x.device_id)
         if residual is not None and residual.shape != x.shape:
             raise ValueError(f"residual must be {x.shape}, got {residual.shape}")
+        ops._apart(out, self.router, self.up, self.down)
         o = ops._result(out, x.shape, x.dtype, x.device_id, "out")
         flat = ops.dev_reshape(x, (math.prod(x.shape[:-1]), self.dim))
         res = ops.dev_reshape(residual, flat.shape) if residual is not None else None

@@ -311,6 +311,12 @@ def test_modules_write_into_kept_results(ops, engine):
     for bad in (_fake(ops, (20, 64), F16), _fake(ops, (4, 5, 64))):
         with pytest.raises(ValueError, match="out must be"):
             m(x, out=bad)
+    for name in ("router", "up", "down"):  # read before the result is written, but kept by the layer
+        kept = getattr(m, name)
+        setattr(m, name, ops.GpuTensor(ops.CudaBuffer(500, 64, 0, False), kept.shape, F16, 0))
+        with pytest.raises(ValueError, match="share memory"):
+            m(x, out=out)
+        setattr(m, name, kept)
     engine.patch("sf_linear_w4", lambda *a: engine.note("y", a[13]))
     lin = nn.Linear4(_w4(ops, N=64))
     x = ops.GpuTensor(ops.CudaBuffer(1 << 16, 4096, 0, False), (4, 5, 256), F16, 0)
