@@ -508,11 +508,14 @@ def dev_moe_route(gt_logits: GpuTensor, top_k: int, renormalize: bool = True,
         out = MoeRoute(_alloc((T, k), i32, dev), _alloc((T, k), np.float32, dev),
                        _alloc((X + 1,), i32, dev), _alloc((T * k,), i32, dev), _alloc((T, k), i32, dev))
     else:
-        _same_device(gt_logits, out.experts, out.weights, out.offsets, out.rows, out.slots)
-        for name, shape in (("experts", (T, k)), ("weights", (T, k)), ("offsets", (X + 1,)),
-                            ("rows", (T * k,)), ("slots", (T, k))):
-            _result(getattr(out, name), shape, _F32 if name == "weights" else _I32, dev, name)
-        _apart(gt_logits, out.experts, out.weights, out.offsets, out.rows, out.slots)
+        e, w, o, r, s = out.experts, out.weights, out.offsets, out.rows, out.slots
+        _same_device(gt_logits, e, w, o, r, s)
+        if not (e.shape == w.shape == s.shape == (T, k) and o.shape == (X + 1,) and r.shape == (T * k,)
+                and e.dtype == o.dtype == r.dtype == s.dtype == _I32 and w.dtype == _F32):
+            for name, t, shape in (("experts", e, (T, k)), ("weights", w, (T, k)), ("offsets", o, (X + 1,)),
+                                   ("rows", r, (T * k,)), ("slots", s, (T, k))):
+                _result(t, shape, _F32 if name == "weights" else _I32, dev, name)
+        _apart(gt_logits, e, w, o, r, s)
     if need and (out.scratch is None or out.scratch.nbytes < need or out.scratch.device_id != dev):
         out.scratch = _make_buffer(need, dev)
     ws = out.scratch.ptr if need else None
@@ -563,25 +566,19 @@ def dev_grouped_linear(gt_x: GpuTensor, gt_weight: GpuTensor, gt_offsets: GpuTen
     y = _result(out, (M, N), odt, dev, "out")
     bias_dt = E.dtype_code(gt_bias.dtype) if gt_bias is not None else DT_F32
     stream, code = E.get_stream(dev), E.dtype_code(gt_x.dtype)
-
-    def launch(ws, ws_bytes):
-        check(lib.sf_gemm_grouped(X, M, N, K, _ptr(gt_x), gt_x.shape[0], K, _ptr(rows),
-                                  _ptr(gt_offsets), _ptr(gt_weight), K, wide * K, _ptr(gt_bias),
-                                  bias_dt, wide, _ptr(y), N, code, E.dtype_code(odt), act, ws,
-                                  ws_bytes, stream),
-              "sf_gemm_grouped")
-
+    call = (X, M, N, K, _ptr(gt_x), gt_x.shape[0], K, _ptr(rows), _ptr(gt_offsets), _ptr(gt_weight),
+            K, wide * K, _ptr(gt_bias), bias_dt, wide, _ptr(y), N, code, E.dtype_code(odt), act)
     with E.on_device(dev):
+        if rows is None or M <= 1024:  # short batches need no workspace
+            check(lib.sf_gemm_grouped(*call, None, 0, stream), "sf_gemm_grouped")
+            return y
         need = C.c_size_t()
-        if rows is not None and M > 1024:  # short batches need none
-            check(lib.sf_gemm_grouped_workspace_size(X, M, N, K, code, stream, C.byref(need)),
-                  "sf_gemm_grouped_workspace_size")
-        if need.value:
-            with E.workspace_lock:
-                buf = E.workspace(dev, stream, need.value)
-                launch(buf.ptr, buf.nbytes)
-        else:
-            launch(None, 0)
+        check(lib.sf_gemm_grouped_workspace_size(X, M, N, K, code, stream, C.byref(need)),
+              "sf_gemm_grouped_workspace_size")
+        with E.workspace_lock:
+            buf = E.workspace(dev, stream, need.value)
+            ws, ws_bytes = (buf.ptr, buf.nbytes) if buf is not None else (None, 0)
+            check(lib.sf_gemm_grouped(*call, ws, ws_bytes, stream), "sf_gemm_grouped")
     return y
 
 
