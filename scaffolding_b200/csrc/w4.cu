@@ -312,7 +312,7 @@ int32_t encode_words(CUtensorMap* m, const W4Args& a, CUtensorMapSwizzle swizzle
 // CTAs per 128 rows of the streaming kernel: the largest cluster with which all
 // clusters run at once, since a second wave costs as much as the first.  The
 // launch before this one leaves its places one by one, so a sixteenth is kept
-// free.  8192 -> 11008, one row: 38.6 / 32.3 / 23.8 / 19.4 / 17.0 / 15.4 us in
+// free.  8192 -> 11008, one row: 38.6 / 32.3 / 23.8 / 19.4 / 17.0 / 15.1 us in
 // clusters of 1 to 6, 19.9 in 8 (two waves); 5120 -> 14336: 14.2 in 4, 16.8 in 5,
 // which fill the device to the last place.  Where nothing fits, the fewest that
 // are more than two per SM (8192 -> 28672, one row: 62.6 / 34.9 / 37.4 / 35.9 us
@@ -327,9 +327,9 @@ int least_stream_splits(int64_t tiles, int sm_count) {
 // its CTA-wide pipeline cost about 3 us more to start and to end than the ring
 // kernel's, and it streams faster, with 9 to 16 rows by more.  Ring / stream,
 // groups of 128, one row of x: 6.7 / 8.0 us at 4096 -> 8192 (2048 blocks), 9.8 /
-// 10.2 us at 4096 -> 11008 (2752), 16.7 / 15.2 us at 4096 -> 22016 (5504), 38.6 /
-// 34.6 us at 8192 -> 28672 (14336); 16 rows: 6.7 / 10.2 us at 4096 x 4096 (1024),
-// 13.0 / 11.6, 18.7 / 15.3, 31.2 / 23.0, 68.9 / 51.0 us.  And it needs its CTAs: one
+// 10.2 us at 4096 -> 11008 (2752), 16.7 / 14.9 us at 4096 -> 22016 (5504), 38.6 /
+// 34.5 us at 8192 -> 28672 (14336); 16 rows: 6.7 / 10.2 us at 4096 x 4096 (1024),
+// 13.0 / 11.4, 18.7 / 15.1, 31.2 / 22.6, 68.9 / 51.3 us.  And it needs its CTAs: one
 // row 13.0 / 19.0 us at 16384 -> 4096, where clusters of 8 are 256 of them.
 constexpr int64_t kStreamBlocks = 4096, kStreamBlocks16 = 2048;
 
@@ -450,7 +450,7 @@ int32_t launch_w4_tc(const W4Args& a, const DeviceInfo& dev, int device, cudaStr
                         mx, a, splits, n_rows, dev.err_word);
 }
 
-// Up to 16 rows of x run on mma.sync, more on tcgen05 (33 rows: 71 us at 8192 ->
+// Up to 16 rows of x run on mma.sync, more on tcgen05 (33 rows: 70 us at 8192 ->
 // 28672, 213 in three passes of the ring kernel).  Rows of x that TMA cannot
 // describe take the ring kernel.
 template <bool BF16>
